@@ -468,6 +468,187 @@ RAC_EXPORT int rac_softmax_dev(const float* x, float* y, long rows, long n, int 
     return check_hip(softmax_launch(x, y, rows, n, iters, (hipStream_t)stream), "rac_softmax_dev launch");
 }
 
+// ── packed prompts, drafted tokens, given tokens (rac_llm.h) ────────────
+
+static bool rows_aligned(const void* p, int es, int d, long s0, long s1, long s2 = 0) {
+    const long v = 16 / es;
+    return (uintptr_t)p % 16 == 0 && d % v == 0 && s0 % v == 0 && s1 % v == 0 && s2 % v == 0;
+}
+
+// the checks that the two attentions share
+static int check_heads(const char* who, int n_heads, int n_kv_heads, int d_head, float scale, int dtype) {
+    if (n_heads <= 0 || n_kv_heads <= 0 || n_heads % n_kv_heads || n_heads > 65535)
+        return fail(RAC_ERR_INVALID_DIM, "%s: n_heads must be a positive multiple of n_kv_heads, at most 65535", who);
+    if (d_head <= 0 || d_head > kPackedMaxHead)
+        return fail(RAC_ERR_INVALID_DIM, "%s: d_head must be in [1, %d]", who, kPackedMaxHead);
+    if (!(scale > 0.0f) || !isfinite(scale)) return fail(RAC_ERR_INVALID_DIM, "%s: scale must be positive", who);
+    if (dtype < 0 || dtype > 2) return fail(RAC_ERR_INVALID_DIM, "%s: dtype must be 0 (fp32), 1 (bf16) or 2 (fp16)", who);
+    return RAC_OK;
+}
+
+static int packed_args(const char* who, PackedArgs* a, int dtype) {
+    int rc = check_heads(who, a->heads, a->kv_heads, a->d, a->scale, dtype);
+    if (rc) return rc;
+    if (a->n_seqs < 0 || a->total < 0 || a->total > (1 << 30))
+        return fail(RAC_ERR_INVALID_DIM, "%s: n_seqs and total must not be negative, total at most 2^30", who);
+    if (((long)a->total / 128 + a->n_seqs + 2) * a->heads > 2147483647L)
+        return fail(RAC_ERR_INVALID_DIM, "%s: too many sequences and heads", who);
+    if (a->sq_t < 0 || a->sq_h < 0 || a->sk_t < 0 || a->sk_h < 0 || a->sv_t < 0 || a->sv_h < 0)
+        return fail(RAC_ERR_INVALID_DIM, "%s: strides must not be negative", who);
+    const int es = dtype == 0 ? 4 : 2;
+    a->vec = rows_aligned(a->q, es, a->d, a->sq_t, a->sq_h) && rows_aligned(a->k, es, a->d, a->sk_t, a->sk_h) &&
+             rows_aligned(a->v, es, a->d, a->sv_t, a->sv_h);
+    return RAC_OK;
+}
+
+RAC_EXPORT int rac_packed_attention_dev(const void* q, const void* k, const void* v, void* out, float* lse,
+                                        const int* cu_seqlens, int n_seqs, int total, int n_heads, int n_kv_heads,
+                                        int d_head, long q_stride, long q_head_stride, long k_stride,
+                                        long k_head_stride, long v_stride, long v_head_stride, float scale,
+                                        int zero_rest, int dtype, void* stream) {
+    const char* who = "rac_packed_attention_dev";
+    if (!q || !k || !v || !out || !cu_seqlens) return fail(RAC_ERR_NULL_PTR, "%s: null buffer", who);
+    PackedArgs a{q, k, v, nullptr, out, nullptr, nullptr, nullptr, lse, nullptr, cu_seqlens, n_seqs, total, n_heads,
+                 n_kv_heads, d_head, q_stride, q_head_stride, k_stride, k_head_stride, v_stride, v_head_stride, scale,
+                 zero_rest, false, false};
+    const int rc = packed_args(who, &a, dtype);
+    if (rc) return rc;
+    const int es = dtype == 0 ? 4 : 2;
+    a.vec_out = (uintptr_t)out % (4 * es) == 0 && d_head % 4 == 0;
+    if (total == 0) return RAC_OK;
+    return check_hip(packed_attention_launch(a, dtype, false, (hipStream_t)stream), "rac_packed_attention_dev launch");
+}
+
+RAC_EXPORT long rac_packed_attention_backward_workspace_bytes(int total, int n_heads) {
+    return total > 0 && n_heads > 0 ? 4L * total * n_heads : 0;
+}
+
+RAC_EXPORT int rac_packed_attention_backward_dev(const void* q, const void* k, const void* v, const void* out,
+                                                 const void* grad_out, const float* lse, const int* cu_seqlens,
+                                                 void* dq, void* dk, void* dv, float* workspace, int n_seqs, int total,
+                                                 int n_heads, int n_kv_heads, int d_head, long q_stride,
+                                                 long q_head_stride, long k_stride, long k_head_stride, long v_stride,
+                                                 long v_head_stride, float scale, int zero_rest, int dtype,
+                                                 void* stream) {
+    const char* who = "rac_packed_attention_backward_dev";
+    if (!q || !k || !v || !out || !grad_out || !lse || !cu_seqlens || !dq || !dk || !dv || !workspace)
+        return fail(RAC_ERR_NULL_PTR, "%s: null buffer", who);
+    PackedArgs a{q, k, v, grad_out, const_cast<void*>(out), dq, dk, dv, const_cast<float*>(lse), workspace, cu_seqlens,
+                 n_seqs, total, n_heads, n_kv_heads, d_head, q_stride, q_head_stride, k_stride, k_head_stride, v_stride,
+                 v_head_stride, scale, zero_rest, false, false};
+    const int rc = packed_args(who, &a, dtype);
+    if (rc) return rc;
+    const int es = dtype == 0 ? 4 : 2;
+    a.vec = a.vec && rows_aligned(out, es, d_head, 0, 0) && rows_aligned(grad_out, es, d_head, 0, 0);
+    a.vec_out = ((uintptr_t)dq | (uintptr_t)dk | (uintptr_t)dv) % (4 * es) == 0 && d_head % 4 == 0;
+    if (total == 0) return RAC_OK;
+    return check_hip(packed_attention_launch(a, dtype, true, (hipStream_t)stream),
+                     "rac_packed_attention_backward_dev launch");
+}
+
+static int tree_args(const char* who, const TreeArgs& a, int dtype) {
+    int rc = check_heads(who, a.heads, a.kv_heads, a.d, a.scale, dtype);
+    if (rc) return rc;
+    if (a.batch < 0 || (long)a.batch * a.kv_heads > 65535)
+        return fail(RAC_ERR_INVALID_DIM, "%s: batch * n_kv_heads must be in [0, 65535]", who);
+    if (a.tokens < 1 || a.tokens > kTreeMaxTokens)
+        return fail(RAC_ERR_INVALID_DIM, "%s: tokens must be in [1, %d]", who, kTreeMaxTokens);
+    if (a.cap < a.tokens || a.cap > 2147483647L - 65536)
+        return fail(RAC_ERR_INVALID_DIM, "%s: t_cap must hold the tokens and stay below 2^31 - 65536", who);
+    if ((long)a.heads / a.kv_heads * a.tokens > 65535L * 32)
+        return fail(RAC_ERR_INVALID_DIM, "%s: too many query rows of a key / value head", who);
+    return RAC_OK;
+}
+
+RAC_EXPORT long rac_tree_attention_workspace_bytes(int batch, int tokens, int n_heads, int n_kv_heads, int d_head,
+                                                   long t_cap, int dtype) {
+    TreeArgs a{};
+    a.batch = batch;
+    a.tokens = tokens;
+    a.heads = n_heads;
+    a.kv_heads = n_kv_heads;
+    a.d = d_head;
+    a.cap = t_cap;
+    a.scale = 1.0f;
+    if (tree_args("rac_tree_attention_workspace_bytes", a, dtype)) return 0;
+    return batch ? tree_attention_workspace(a, dtype) : 0;
+}
+
+RAC_EXPORT int rac_tree_attention_dev(const void* q, const void* k_cache, const void* v_cache, void* out,
+                                      const int* lengths, const int* parents, float* workspace, int batch, int tokens,
+                                      int n_heads, int n_kv_heads, int d_head, long t_cap, long parents_stride,
+                                      long q_stride_b, long q_stride_t, long q_stride_h, long k_stride_b,
+                                      long k_stride_h, long k_stride_t, long v_stride_b, long v_stride_h,
+                                      long v_stride_t, float scale, int dtype, void* stream) {
+    const char* who = "rac_tree_attention_dev";
+    if (!q || !k_cache || !v_cache || !out || !lengths || !parents)
+        return fail(RAC_ERR_NULL_PTR, "%s: null buffer", who);
+    TreeArgs a{q, k_cache, v_cache, out, workspace, lengths, parents, batch, tokens, n_heads, n_kv_heads, d_head, 1,
+               t_cap, parents_stride, q_stride_b, q_stride_t, q_stride_h, k_stride_b, k_stride_h, k_stride_t,
+               v_stride_b, v_stride_h, v_stride_t, scale, false, false};
+    const int rc = tree_args(who, a, dtype);
+    if (rc) return rc;
+    if (parents_stride < 0 || q_stride_b < 0 || q_stride_t < 0 || q_stride_h < 0 || k_stride_b < 0 || k_stride_h < 0 ||
+        k_stride_t < 0 || v_stride_b < 0 || v_stride_h < 0 || v_stride_t < 0)
+        return fail(RAC_ERR_INVALID_DIM, "%s: strides must not be negative", who);
+    if (batch == 0) return RAC_OK;
+    if (!workspace && tree_attention_workspace(a, dtype) > 0) return fail(RAC_ERR_NULL_PTR, "%s: null workspace", who);
+    const int es = dtype == 0 ? 4 : 2;
+    a.vec = rows_aligned(q, es, d_head, q_stride_b, q_stride_t, q_stride_h) &&
+            rows_aligned(k_cache, es, d_head, k_stride_b, k_stride_h, k_stride_t) &&
+            rows_aligned(v_cache, es, d_head, v_stride_b, v_stride_h, v_stride_t);
+    a.vec_out = (uintptr_t)out % (4 * es) == 0 && d_head % 4 == 0;
+    return check_hip(tree_attention_launch(a, dtype, (hipStream_t)stream), "rac_tree_attention_dev launch");
+}
+
+static int check_logits(const char* who, long rows, long vocab, long row_stride, int dtype) {
+    if (rows < 0 || rows > 2147483647L) return fail(RAC_ERR_INVALID_DIM, "%s: rows must be in [0, 2^31 - 1]", who);
+    if (vocab < 1 || vocab > 2147483647L - 64) return fail(RAC_ERR_INVALID_DIM, "%s: vocab must be in [1, 2^31 - 65]", who);
+    if (row_stride < vocab && rows > 1)
+        return fail(RAC_ERR_INVALID_DIM, "%s: row_stride must be at least vocab", who);
+    if (dtype < 0 || dtype > 2) return fail(RAC_ERR_INVALID_DIM, "%s: dtype must be 0 (fp32), 1 (bf16) or 2 (fp16)", who);
+    return RAC_OK;
+}
+
+RAC_EXPORT long rac_token_logprobs_workspace_bytes(long rows, long vocab, int top, int dtype) {
+    if (rows <= 0 || top < 0 || top > kLogprobMaxTop ||
+        check_logits("rac_token_logprobs_workspace_bytes", rows, vocab, vocab, dtype))
+        return 0;
+    return token_logprobs_workspace(rows, vocab, top, dtype);
+}
+
+RAC_EXPORT int rac_token_logprobs_dev(const void* logits, long row_stride, const long* tokens, float* logprob,
+                                      float* entropy, float* lse, float* top_logprob, long* top_token,
+                                      float* workspace, long rows, long vocab, int top, int dtype, void* stream) {
+    const char* who = "rac_token_logprobs_dev";
+    if (!logits || !tokens || !logprob || !entropy) return fail(RAC_ERR_NULL_PTR, "%s: null buffer", who);
+    const int rc = check_logits(who, rows, vocab, row_stride, dtype);
+    if (rc) return rc;
+    if (top < 0 || top > kLogprobMaxTop || top > vocab)
+        return fail(RAC_ERR_INVALID_DIM, "%s: top must be in [0, min(%d, vocab)]", who, kLogprobMaxTop);
+    if (top && (!top_logprob || !top_token)) return fail(RAC_ERR_NULL_PTR, "%s: null top buffer", who);
+    if (rows == 0) return RAC_OK;
+    if (!workspace && token_logprobs_workspace(rows, vocab, top, dtype) > 0)
+        return fail(RAC_ERR_NULL_PTR, "%s: null workspace", who);
+    LogprobArgs a{logits, tokens, logprob, entropy, lse, top_logprob, workspace, top_token, rows, vocab, row_stride, top, 1};
+    return check_hip(token_logprobs_launch(a, dtype, (hipStream_t)stream), "rac_token_logprobs_dev launch");
+}
+
+RAC_EXPORT int rac_token_logprobs_backward_dev(const void* logits, long row_stride, const long* tokens,
+                                               const float* lse, const float* entropy, const float* grad_logprob,
+                                               const float* grad_entropy, void* grad_logits, long rows, long vocab,
+                                               int dtype, void* stream) {
+    const char* who = "rac_token_logprobs_backward_dev";
+    if (!logits || !tokens || !lse || !entropy || !grad_logits || (!grad_logprob && !grad_entropy))
+        return fail(RAC_ERR_NULL_PTR, "%s: null buffer", who);
+    const int rc = check_logits(who, rows, vocab, row_stride, dtype);
+    if (rc) return rc;
+    if (rows == 0) return RAC_OK;
+    return check_hip(token_logprobs_backward_launch(logits, row_stride, tokens, lse, entropy, grad_logprob,
+                                                    grad_entropy, grad_logits, rows, vocab, dtype, (hipStream_t)stream),
+                     "rac_token_logprobs_backward_dev launch");
+}
+
 // ── decode step (bench_rac_transformer.c decoder_forward_kv, T_new = 1) ──
 
 // Grouped-query attention of one token over positions 0 .. *pos of the

@@ -183,6 +183,58 @@ hipError_t kv_append_launch(const float* kv, float* kc, float* vc, int n_kv_head
                             const int* pos, hipStream_t s);
 hipError_t position_advance_launch(int* pos, int by, hipStream_t s);
 hipError_t swiglu_launch(const float* gu, float* out, long n, int iters, hipStream_t s);
+// Causal attention over packed sequences (rac_packed.hip): q [total, heads, d],
+// k and v [total, kv_heads, d] with element strides per row (_t) and head (_h);
+// out, grad, dq [total, heads, d], dk, dv [total, kv_heads, d] contiguous; lse,
+// delta [heads, total].  vec: every row of q, k, v (and out, grad in a backward
+// pass) is 16-byte aligned and d whole 16-byte vectors; vec_out: the outputs'
+// rows take stores of 4 values.  zero_rest: rows outside every sequence become 0.
+// dtype 0 fp32, 1 bf16, 2 fp16; d <= kPackedMaxHead.
+constexpr int kPackedMaxHead = 256;
+struct PackedArgs {
+    const void *q, *k, *v, *grad;
+    void *out, *dq, *dk, *dv;
+    float *lse, *delta;
+    const int* cu;
+    int n_seqs, total, heads, kv_heads, d;
+    long sq_t, sq_h, sk_t, sk_h, sv_t, sv_h;
+    float scale;
+    int zero_rest;
+    bool vec, vec_out;
+};
+hipError_t packed_attention_launch(const PackedArgs& a, int dtype, bool backward, hipStream_t s);
+// Attention of drafted tokens over a cache (rac_tree.hip): q [batch, tokens,
+// heads, d], caches [batch, kv_heads, cap, d], element strides; out contiguous
+// [batch, tokens, heads, d]; part: tree_attention_workspace bytes.
+constexpr int kTreeMaxTokens = 256;
+struct TreeArgs {
+    const void *q, *k, *v;
+    void* out;
+    float* part;
+    const int *len, *parents;
+    int batch, tokens, heads, kv_heads, d, splits;
+    long cap, parents_b, sq_b, sq_t, sq_h, sk_b, sk_g, sk_t, sv_b, sv_g, sv_t;
+    float scale;
+    bool vec, vec_out;
+};
+long tree_attention_workspace(const TreeArgs& a, int dtype);
+hipError_t tree_attention_launch(TreeArgs a, int dtype, hipStream_t s);
+// Log probabilities of given tokens (rac_logprob.hip): rows of `vocab` logits
+// `stride` elements apart; lse, entropy, top_lp, top_tok may be null (top 0).
+constexpr int kLogprobMaxTop = 64;
+struct LogprobArgs {
+    const void* x;
+    const long* tok;
+    float *lp, *ent, *lse, *top_lp, *part;
+    long *top_tok;
+    long rows, vocab, stride;
+    int top, splits;
+};
+long token_logprobs_workspace(long rows, long vocab, int top, int dtype);
+hipError_t token_logprobs_launch(LogprobArgs a, int dtype, hipStream_t s);
+hipError_t token_logprobs_backward_launch(const void* x, long stride, const long* tok, const float* lse,
+                                          const float* ent, const float* g_lp, const float* g_ent, void* dx, long rows,
+                                          long vocab, int dtype, hipStream_t s);
 hipError_t q8_dequantize_launch(const uint8_t* src, float* dst, long nblocks, hipStream_t s);
 // Error channel of the C ABI (rac_last_error): set the message, return code.
 int report(int code, const char* fmt, ...) __attribute__((format(printf, 2, 3)));

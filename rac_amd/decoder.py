@@ -131,6 +131,7 @@ class RACDecoder:
         self.length = 0
         self.pos = torch.zeros(1, device=dev, dtype=torch.int32)     # the length, on the device
         self._graph = None
+        self._draft = None
         # the fused decode GEMVs (norm inside, cache / SwiGLU epilogues) need
         # d_model % 256 == 0 and 16-byte aligned buffers; other shapes run
         # the same arithmetic unfused
@@ -144,6 +145,7 @@ class RACDecoder:
         """kv_reset (:492): the cache is empty again."""
         self.length = 0
         self.pos.zero_()
+        self._draft = None
 
     def _linear(self, x: torch.Tensor, w: torch.Tensor, act: int = 0) -> torch.Tensor:
         return ext.fused_linear_forward(x, w, None, act, iters=self.iters, mode=ext.MODE_FAST)
@@ -226,6 +228,7 @@ class RACDecoder:
         if self.length >= self.t_max:
             raise RuntimeError("RAC: KV cache full")
         dev = self.pos.device
+        self._draft = None
         x0 = torch.zeros((1, self.cfg.d_model), device=dev)
         self._decode_step(x0)
         self.pos.fill_(self.length)
@@ -255,6 +258,7 @@ class RACDecoder:
         if T > 1 and self.layers[0].f32 is None:
             raise RuntimeError("RAC: prefill needs the fp32 weights (keep_f32=True)")
         start = self.length
+        self._draft = None
         x = x.contiguous()
         if T == 1:
             if x.data_ptr() % 16:
@@ -277,6 +281,64 @@ class RACDecoder:
         if x.dim() != 2 or x.size(0) != 1:
             raise RuntimeError("RAC: step expects x of shape [1, d_model]")
         return self.forward(x)
+
+    @torch.no_grad()
+    def verify(self, x: torch.Tensor, parents) -> torch.Tensor:
+        """A tree of drafted tokens x [T, d_model] in one pass over the decode
+        weights: token t continues token parents[t] < t or the cache itself
+        (-1).  Returns the stack's output [T, d_model], for each token what
+        step() would give after its ancestors, up to the order of the
+        attention's sums.  The drafts wait behind the cache's end: accept()
+        takes a path of them into the cache, any other call drops them."""
+        cfg = self.cfg
+        parents = [int(p) for p in parents]
+        T = len(parents)
+        if x.dim() != 2 or tuple(x.shape) != (T, cfg.d_model) or x.dtype != torch.float32:
+            raise RuntimeError("RAC: verify expects fp32 x of shape [T, d_model] and T parents")
+        if not 1 <= T <= ext.TREE_MAX_TOKENS:
+            raise RuntimeError(f"RAC: a tree has 1 to {ext.TREE_MAX_TOKENS} tokens")
+        if any(not -1 <= p < t for t, p in enumerate(parents)):
+            raise RuntimeError("RAC: a drafted token continues an earlier one or -1")
+        if self.length + T > self.t_max:
+            raise RuntimeError("RAC: KV cache full")
+        d, dh, nkv = cfg.d_model, cfg.d_head, cfg.n_kv_heads
+        at = slice(self.length, self.length + T)
+        tree = torch.tensor(parents, device=x.device, dtype=torch.int32)
+        x = x.contiguous()
+        for L, lw in enumerate(self.layers):
+            qkv = ext.q8_gemv(ext.rmsnorm(x, lw.rms_att, cfg.eps), lw.q8_qkv)
+            self.k_cache[L][:, at] = qkv[:, d:d + nkv * dh].reshape(T, nkv, dh).transpose(0, 1)
+            self.v_cache[L][:, at] = qkv[:, d + nkv * dh:].reshape(T, nkv, dh).transpose(0, 1)
+            att = ext.tree_attention(qkv[:, :d].unflatten(1, (cfg.n_heads, dh)), self.k_cache[L], self.v_cache[L],
+                                     self.pos, tree, self.scale)
+            x = x + ext.q8_gemv(att.view(T, d), lw.q8_o)
+            gu = ext.q8_gemv(ext.rmsnorm(x, lw.rms_ffn, cfg.eps), lw.q8_gu).view(T, cfg.d_ff, 2)
+            f = ext.silu(gu[..., 0], self.iters) * gu[..., 1]
+            x = x + ext.q8_gemv(f, lw.q8_d)
+        self._draft = (self.length, parents)
+        return x
+
+    @torch.no_grad()
+    def accept(self, path) -> None:
+        """Takes drafted tokens of the last verify() into the cache: path is a
+        run of tokens from a root on, each continuing the one before (it may be
+        empty).  Their keys and values move up to the cache's end and the
+        length advances."""
+        path = [int(t) for t in path]
+        if self._draft is None or self._draft[0] != self.length:
+            raise RuntimeError("RAC: accept follows verify")
+        parents = self._draft[1]
+        for before, t in zip([-1] + path, path):
+            if not 0 <= t < len(parents) or parents[t] != before:
+                raise RuntimeError("RAC: accept takes a path of the tree from one of its roots")
+        n = len(path)
+        if path != list(range(n)):
+            at = torch.tensor(path, device=self.pos.device) + self.length
+            for c in self.k_cache + self.v_cache:
+                c[:, self.length:self.length + n] = c.index_select(1, at)
+        self._draft = None
+        self.length += n
+        self.pos.fill_(self.length)
 
     @staticmethod
     def synthetic_weights(cfg: DecoderConfig, device, seed: int = 0) -> List[dict]:

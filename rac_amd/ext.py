@@ -9,7 +9,8 @@ rac_torch_bind.cpp:54-55) and argument checks.  Added ops (new names, so the
 reference's ``hasattr`` probing keeps working): ``rope_cache``,
 ``rope_apply_``, ``softmax``, ``rmsnorm``, ``layernorm``, ``silu``, ``gelu``,
 ``sigmoid``, ``tanh``, ``exp``, ``relu``, ``rsqrt``, ``sincos``, ``bmm``,
-``softmax_masked_``, ``attention``, and the rac.h vector primitives
+``softmax_masked_``, ``attention``, ``packed_attention``,
+``tree_attention``, ``token_logprobs``, and the rac.h vector primitives
 ``vec2``, ``inner``, ``outer``, ``dct``.
 
 Every op launches on torch's current HIP stream of the tensor's device and
@@ -1064,6 +1065,255 @@ def swiglu(gu: torch.Tensor, iters: int = 0) -> torch.Tensor:
     return out
 
 
+# ── packed prompts, drafted tokens, given tokens (rac_llm.h) ────────────────
+
+LLM_MAX_HEAD = 256
+TREE_MAX_TOKENS = 256
+LOGPROB_MAX_TOP = 64
+_LLM_DTYPE = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+
+
+def _llm_dtype(t: torch.Tensor, what: str) -> int:
+    _require_gpu(t, what)
+    if t.dtype not in _LLM_DTYPE:
+        raise RuntimeError(f"RAC: {what} must be float32, bfloat16 or float16")
+    return _LLM_DTYPE[t.dtype]
+
+
+def _like(t: torch.Tensor, ref: torch.Tensor, what: str) -> None:
+    _require_gpu(t, what)
+    if t.device != ref.device:
+        raise RuntimeError(f"RAC: {what} must be on {ref.device}")
+
+
+def _require_int32(t: torch.Tensor, ref: torch.Tensor, what: str) -> torch.Tensor:
+    _like(t, ref, what)
+    if t.dtype != torch.int32:
+        raise RuntimeError(f"RAC: {what} must be int32")
+    return t.contiguous()
+
+
+def _unit_last(t: torch.Tensor) -> torch.Tensor:
+    """t unchanged when its last dim is contiguous, a contiguous copy otherwise."""
+    return t if t.stride(-1) == 1 or t.size(-1) == 1 else t.contiguous()
+
+
+def _fresh_or(out: Optional[torch.Tensor], shape, ref: torch.Tensor) -> torch.Tensor:
+    if out is None:
+        return torch.empty(shape, device=ref.device, dtype=ref.dtype)
+    _like(out, ref, "out")
+    if out.dtype != ref.dtype or tuple(out.shape) != tuple(shape) or not out.is_contiguous():
+        raise RuntimeError(f"RAC: out must be a contiguous {ref.dtype} tensor of shape {tuple(shape)}")
+    return out
+
+
+def _call(name: str, ref: torch.Tensor, *args) -> None:
+    """The entry point on ref's device and torch's current stream there."""
+    with torch.cuda.device(ref.device):
+        check(getattr(_lib.load(), name)(*args, _stream(ref)), name)
+
+
+def _packed_checks(q, k, v, cu_seqlens):
+    dt = _llm_dtype(q, "q")
+    for t, n in ((k, "k"), (v, "v")):
+        _like(t, q, n)
+        if t.dtype != q.dtype:
+            raise RuntimeError("RAC: q, k and v must have the same dtype")
+    if q.dim() != 3 or k.dim() != 3 or k.shape != v.shape or q.size(0) != k.size(0) or q.size(2) != k.size(2):
+        raise RuntimeError("RAC: packed_attention expects q [total, n_heads, d_head], k and v "
+                           "[total, n_kv_heads, d_head]")
+    if k.size(1) == 0 or q.size(1) == 0 or q.size(1) % k.size(1):
+        raise RuntimeError("RAC: n_heads must be a multiple of n_kv_heads")
+    if not 0 < q.size(2) <= LLM_MAX_HEAD:
+        raise RuntimeError(f"RAC: d_head must be in [1, {LLM_MAX_HEAD}]")
+    cu = _require_int32(cu_seqlens, q, "cu_seqlens")
+    if cu.dim() != 1 or cu.numel() < 1:
+        raise RuntimeError("RAC: cu_seqlens must be a vector of n_seqs + 1 row numbers")
+    return dt, _unit_last(q), _unit_last(k), _unit_last(v), cu
+
+
+def _packed_tail(q, k, v):
+    return (q.stride(0), q.stride(1), k.stride(0), k.stride(1), v.stride(0), v.stride(1))
+
+
+def packed_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqlens: torch.Tensor,
+                     scale: Optional[float] = None, return_lse: bool = False, out: Optional[torch.Tensor] = None):
+    """Causal attention within each of several sequences packed one behind
+    the other: sequence i is rows cu_seqlens[i] .. cu_seqlens[i + 1] - 1
+    (int32, on the device, non-decreasing; sequences may be empty) of q
+    [total, n_heads, d_head] and k, v [total, n_kv_heads, d_head] in fp32,
+    bf16 or fp16, whose last dim is contiguous and whose others may be strided
+    (slices of a stacked projection).  Query head h reads key / value head
+    h // (n_heads / n_kv_heads); scale defaults to 1 / sqrt(d_head).  Returns
+    [total, n_heads, d_head]; with return_lse also log sum exp of the scores
+    [n_heads, total] (fp32), which packed_attention_backward takes.  Rows
+    outside every sequence are 0, or with `out` stay as they are there (lse
+    there: undefined)."""
+    dt, q, k, v, cu = _packed_checks(q, k, v, cu_seqlens)
+    total, H, D = q.shape
+    fresh = out is None
+    out = _fresh_or(out, q.shape, q)
+    lse = torch.empty((H, total), device=q.device, dtype=torch.float32) if return_lse else None
+    scale = attention_scale(D) if scale is None else float(scale)
+    if total:
+        _call("rac_packed_attention_dev", q, q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(),
+              lse.data_ptr() if lse is not None else None, cu.data_ptr(), cu.numel() - 1, total, H, k.size(1), D,
+              *_packed_tail(q, k, v), scale, int(fresh), dt)
+    return (out, lse) if return_lse else out
+
+
+def packed_attention_backward(grad_out: torch.Tensor, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
+                              out: torch.Tensor, lse: torch.Tensor, cu_seqlens: torch.Tensor,
+                              scale: Optional[float] = None) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    """(dq, dk, dv) of packed_attention, contiguous and in q's dtype, from its
+    output and lse; 0 in rows outside every sequence.  The sums over the query
+    heads of a group run in a fixed order: the same call, the same bits."""
+    dt, q, k, v, cu = _packed_checks(q, k, v, cu_seqlens)
+    total, H, D = q.shape
+    for t, n in ((grad_out, "grad_out"), (out, "out")):
+        _like(t, q, n)
+        if t.shape != q.shape or t.dtype != q.dtype:
+            raise RuntimeError(f"RAC: {n} must have q's shape and dtype")
+    _like(lse, q, "lse")
+    if lse.dtype != torch.float32 or tuple(lse.shape) != (H, total) or not lse.is_contiguous():
+        raise RuntimeError("RAC: lse must be the contiguous fp32 [n_heads, total] of packed_attention")
+    grad_out, out = grad_out.contiguous(), out.contiguous()
+    dq = torch.empty(q.shape, device=q.device, dtype=q.dtype)
+    dk, dv = (torch.empty(k.shape, device=q.device, dtype=q.dtype) for _ in range(2))
+    scale = attention_scale(D) if scale is None else float(scale)
+    if total:
+        ws = torch.empty(_lib.load().rac_packed_attention_backward_workspace_bytes(total, H) // 4, device=q.device,
+                         dtype=torch.float32)
+        _call("rac_packed_attention_backward_dev", q, q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(),
+              grad_out.data_ptr(), lse.data_ptr(), cu.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(),
+              ws.data_ptr(), cu.numel() - 1, total, H, k.size(1), D, *_packed_tail(q, k, v), scale, 1, dt)
+    return dq, dk, dv
+
+
+def tree_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, lengths: torch.Tensor,
+                   parents: torch.Tensor, scale: Optional[float] = None,
+                   out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Attention of drafted tokens over a key/value cache: q [batch, T,
+    n_heads, d_head], caches [batch, n_kv_heads, t_cap, d_head] in fp32, bf16
+    or fp16 (last dims contiguous, others may be strided).  Sequence b's cache
+    holds lengths[b] tokens and, at the T positions behind them, the drafted
+    tokens' keys and values; drafted token t continues token parents[b, t] < t
+    or, with -1, the cache itself, and sees the cache, its ancestors and
+    itself.  parents [T] is one tree for all.  lengths and parents (int32) are
+    read on the device when the kernels run: a recorded graph replays with new
+    ones.  Without the batch dim (q [T, n_heads, d_head], caches [n_kv_heads,
+    t_cap, d_head], one length): one sequence.  T <= 256.  Returns q's shape;
+    NaN for a sequence whose length does not leave T positions."""
+    single = isinstance(q, torch.Tensor) and q.dim() == 3
+    dt = _llm_dtype(q, "q")
+    for t, n in ((k_cache, "k_cache"), (v_cache, "v_cache")):
+        _like(t, q, n)
+        if t.dtype != q.dtype:
+            raise RuntimeError("RAC: q and the caches must have the same dtype")
+    if single:
+        q, k_cache, v_cache = q.unsqueeze(0), k_cache.unsqueeze(0), v_cache.unsqueeze(0)
+    if q.dim() != 4 or k_cache.dim() != 4 or k_cache.shape != v_cache.shape or q.size(0) != k_cache.size(0) \
+            or q.size(3) != k_cache.size(3):
+        raise RuntimeError("RAC: tree_attention expects q [batch, T, n_heads, d_head] and caches "
+                           "[batch, n_kv_heads, t_cap, d_head]")
+    B, T, H, D = q.shape
+    G, cap = k_cache.size(1), k_cache.size(2)
+    if G == 0 or H == 0 or H % G:
+        raise RuntimeError("RAC: n_heads must be a multiple of n_kv_heads")
+    if not 0 < D <= LLM_MAX_HEAD:
+        raise RuntimeError(f"RAC: d_head must be in [1, {LLM_MAX_HEAD}]")
+    if not 1 <= T <= TREE_MAX_TOKENS:
+        raise RuntimeError(f"RAC: a tree has 1 to {TREE_MAX_TOKENS} tokens")
+    lengths = _require_int32(lengths, q, "lengths")
+    parents = _require_int32(parents, q, "parents")
+    if lengths.numel() != B:
+        raise RuntimeError("RAC: lengths must hold one length per sequence")
+    if tuple(parents.shape) not in ((T,), (B, T)):
+        raise RuntimeError("RAC: parents must be [T] or [batch, T]")
+    q, k, v = _unit_last(q), _unit_last(k_cache), _unit_last(v_cache)
+    res = _fresh_or(out, (T, H, D) if single else (B, T, H, D), q)
+    scale = attention_scale(D) if scale is None else float(scale)
+    if B:
+        n = _lib.load().rac_tree_attention_workspace_bytes(B, T, H, G, D, cap, dt)
+        ws = torch.empty(n // 4, device=q.device, dtype=torch.float32) if n else None
+        _call("rac_tree_attention_dev", q, q.data_ptr(), k.data_ptr(), v.data_ptr(), res.data_ptr(),
+              lengths.data_ptr(), parents.data_ptr(), ws.data_ptr() if n else None, B, T, H, G, D, cap,
+              T if parents.dim() == 2 else 0, q.stride(0), q.stride(1), q.stride(2), k.stride(0), k.stride(1),
+              k.stride(2), v.stride(0), v.stride(1), v.stride(2), scale, dt)
+    return res
+
+
+def _logit_rows(logits: torch.Tensor, tokens: torch.Tensor):
+    dt = _llm_dtype(logits, "logits")
+    _like(tokens, logits, "tokens")
+    if tokens.dtype not in (torch.int64, torch.int32):
+        raise RuntimeError("RAC: tokens must be int64 or int32")
+    if logits.dim() < 1 or logits.size(-1) < 1 or tokens.shape != logits.shape[:-1]:
+        raise RuntimeError("RAC: tokens must have the shape of logits without its last dim")
+    V = logits.size(-1)
+    x = logits.reshape(-1, V)
+    if (V > 1 and x.stride(1) != 1) or (x.size(0) > 1 and x.stride(0) < V):
+        x = x.contiguous()
+    return dt, x, tokens.reshape(-1).to(torch.int64).contiguous()
+
+
+def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, top: int = 0, return_lse: bool = False):
+    """Of each row of logits [..., vocab] (fp32, bf16 or fp16): the log
+    probability of its given token (tokens [...], int64 or int32; a negative
+    one stands for none and gives 0, one past the vocabulary NaN) and the
+    entropy; with top > 0 also the `top` (<= 64) likeliest tokens' log
+    probabilities and tokens [..., top], best first, equal logits by the lower
+    token; with return_lse also log sum exp.  Returns (logprobs, entropy[,
+    top_logprobs, top_tokens][, lse]), all fp32 but the int64 tokens.  Logits
+    of -inf have no part; a row of nothing else gives -inf and entropy 0."""
+    dt, x, tok = _logit_rows(logits, tokens)
+    N, V = x.shape
+    top = int(top)
+    if not 0 <= top <= min(LOGPROB_MAX_TOP, V):
+        raise RuntimeError(f"RAC: top must be in [0, min({LOGPROB_MAX_TOP}, vocab)]")
+    lead = logits.shape[:-1]
+    f32 = dict(device=x.device, dtype=torch.float32)
+    lp, ent = torch.empty(lead, **f32), torch.empty(lead, **f32)
+    lse = torch.empty(lead, **f32) if return_lse else None
+    tv = torch.empty((*lead, top), **f32) if top else None
+    ti = torch.empty((*lead, top), device=x.device, dtype=torch.int64) if top else None
+    if N:
+        n = _lib.load().rac_token_logprobs_workspace_bytes(N, V, top, dt)
+        ws = torch.empty(n // 4, **f32) if n else None
+        _call("rac_token_logprobs_dev", x, x.data_ptr(), x.stride(0) if N > 1 else V, tok.data_ptr(), lp.data_ptr(),
+              ent.data_ptr(), lse.data_ptr() if return_lse else None, tv.data_ptr() if top else None,
+              ti.data_ptr() if top else None, ws.data_ptr() if n else None, N, V, top, dt)
+    return (lp, ent) + ((tv, ti) if top else ()) + ((lse,) if return_lse else ())
+
+
+def token_logprobs_backward(logits: torch.Tensor, tokens: torch.Tensor, lse: torch.Tensor, entropy: torch.Tensor,
+                            grad_logprobs: Optional[torch.Tensor],
+                            grad_entropy: Optional[torch.Tensor]) -> torch.Tensor:
+    """The gradient of the logits (their shape and dtype, contiguous) from
+    those of token_logprobs' log probabilities and entropy (either may be
+    None) and its lse and entropy."""
+    dt, x, tok = _logit_rows(logits, tokens)
+    N, V = x.shape
+    rows = []
+    for t, n in ((lse, "lse"), (entropy, "entropy"), (grad_logprobs, "grad_logprobs"), (grad_entropy, "grad_entropy")):
+        if t is not None:
+            _like(t, x, n)
+            if t.shape != tokens.shape or t.dtype != torch.float32:
+                raise RuntimeError(f"RAC: {n} must be fp32 of the tokens' shape")
+            t = t.contiguous()
+        elif n in ("lse", "entropy"):
+            raise RuntimeError(f"RAC: {n} is needed")
+        rows.append(t)
+    dx = torch.empty(logits.shape, device=x.device, dtype=x.dtype)
+    if rows[2] is None and rows[3] is None:
+        return dx.zero_()
+    if N:
+        _call("rac_token_logprobs_backward_dev", x, x.data_ptr(), x.stride(0) if N > 1 else V, tok.data_ptr(),
+              rows[0].data_ptr(), rows[1].data_ptr(), rows[2].data_ptr() if rows[2] is not None else None,
+              rows[3].data_ptr() if rows[3] is not None else None, dx.data_ptr(), N, V, dt)
+    return dx
+
+
 # ── RAC-DSP fixed-point engine (sim/rac_dsp_core.h) ──────────────────────
 
 DSP_OPS = {"rotate": 0, "project": 1, "vectoring": 2, "hyperbolic": 3}
@@ -1197,6 +1447,8 @@ __all__ = [
     "rsqrt", "sincos", "rope_inv_freq", "rope_cache", "rope_apply_", "rope_apply",
     "bmm", "softmax_masked_", "attention", "attention_probs_rows", "attention_backward", "vec2", "inner", "outer", "dct", "VEC2_OPS",
     "fused_linear_forward", "fused_linear_backward", "act_grad", "attention_scale",
+    "packed_attention", "packed_attention_backward", "tree_attention", "token_logprobs", "token_logprobs_backward",
+    "LLM_MAX_HEAD", "TREE_MAX_TOKENS", "LOGPROB_MAX_TOP",
     "q8_quantize", "q8_dequantize", "q8_gemv", "Q8_BLOCK_BYTES",
     "dsp_eval", "dsp_systolic", "DSP_OPS", "SafeTensors",
 ]

@@ -32,6 +32,7 @@ from typing import Optional
 import torch
 import torch.nn as nn
 from torch.autograd import Function
+from torch.autograd.function import once_differentiable
 
 from . import _probe
 from . import ext as _rac
@@ -814,6 +815,69 @@ def rac_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, mask: Optio
     """Attention core of [B, H, T, D] tensors through RAC; mask: optional
     additive [T, T]."""
     return RACAttentionFunction.apply(q, k, v, mask, is_causal)
+
+
+class RACPackedAttentionFunction(Function):
+    """Causal attention over packed sequences with grouped heads (fp32, bf16 or
+    fp16 on the matrix cores, whatever rac_set_mode says); backward recomputes
+    the probabilities from the forward pass's log sums."""
+
+    @staticmethod
+    def forward(ctx, q, k, v, cu_seqlens, scale):
+        _need_gpu(q, "q")
+        if not any(ctx.needs_input_grad[:3]):
+            return _rac.packed_attention(q, k, v, cu_seqlens, scale)
+        out, lse = _rac.packed_attention(q, k, v, cu_seqlens, scale, return_lse=True)
+        ctx.save_for_backward(q, k, v, out, lse, cu_seqlens)
+        ctx.scale = scale
+        return out
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, g):
+        q, k, v, out, lse, cu_seqlens = ctx.saved_tensors
+        return (*_rac.packed_attention_backward(g, q, k, v, out, lse, cu_seqlens, ctx.scale), None, None)
+
+
+def rac_packed_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqlens: torch.Tensor,
+                         scale: Optional[float] = None) -> torch.Tensor:
+    """Causal attention within sequences packed one behind the other: q
+    [total, n_heads, d_head], k and v [total, n_kv_heads, d_head], sequence i
+    the rows cu_seqlens[i] .. cu_seqlens[i + 1] - 1 (int32, on the device);
+    ext.packed_attention with gradients."""
+    return RACPackedAttentionFunction.apply(q, k, v, cu_seqlens, scale)
+
+
+class RACTokenLogprobsFunction(Function):
+    """Log probabilities of given tokens and the entropy of rows of logits,
+    with the gradients of both; the top alternatives carry none."""
+
+    @staticmethod
+    def forward(ctx, logits, tokens, top):
+        _need_gpu(logits, "logits")
+        ctx.set_materialize_grads(False)
+        if not ctx.needs_input_grad[0]:
+            return _rac.token_logprobs(logits, tokens, top)
+        *res, lse = _rac.token_logprobs(logits, tokens, top, return_lse=True)
+        ctx.save_for_backward(logits, tokens, lse, res[1])
+        ctx.mark_non_differentiable(*res[2:])
+        return tuple(res)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, g_lp, g_ent, *_):
+        if g_lp is None and g_ent is None:
+            return None, None, None
+        logits, tokens, lse, ent = ctx.saved_tensors
+        return _rac.token_logprobs_backward(logits, tokens, lse, ent, g_lp, g_ent), None, None
+
+
+def rac_token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, top: int = 0):
+    """(log probabilities of `tokens`, entropy) of rows of logits [..., vocab],
+    with top > 0 also (top log probabilities, top tokens); the first two have
+    gradients.  A negative token stands for none (padding): 0 and no gradient.
+    The training loss of next-token prediction is -logprobs.mean()."""
+    return RACTokenLogprobsFunction.apply(logits, tokens, int(top))
 
 
 def _dropout_inactive(dropout: nn.Module) -> bool:
