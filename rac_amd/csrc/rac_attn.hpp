@@ -33,6 +33,120 @@ struct TileStage {
     }
 };
 
+// A tile of rows in LDS: row r's 16-byte vectors lie in it without padding,
+// vector c at place c ^ tile_swz(r), so that both ways of reading a tile, 32
+// rows at the same vector (rows as a left operand) and 4 rows by 32 values
+// (transposed), touch every bank equally often.
+template <int CPR>
+__device__ __forceinline__ int tile_swz(int r) {
+    if constexpr (CPR % 16 == 0) return ((r & 3) << 2) | ((r >> 2) & 3);
+    else if constexpr (CPR % 8 == 0) return (((r >> 1) & 1) << 2) | ((r >> 2) & 3);
+    else return (r >> 2) & 3;
+}
+
+template <typename T, int DP>
+struct Tile {
+    using M = Mma<T>;
+    using Frag = typename M::Frag;
+    static constexpr int RB = DP * (int)sizeof(T), CPR = RB / 16;     // bytes and vectors of a row
+
+    // fragment f of row r of the tile's rows from `row` on (row % 16 == 0), r = lane % 32
+    static __device__ __forceinline__ Frag rows(const char* lds, int row, int f, int lane) {
+        const int r = lane & 31;
+        return *reinterpret_cast<const Frag*>(lds + (row + r) * RB + ((2 * f + (lane >> 5)) ^ tile_swz<CPR>(r)) * 16);
+    }
+    // Mma's transposed fragment f of the 32 rows from `row` on, columns 32 n + lane % 32
+    static __device__ __forceinline__ Frag cols(const char* lds, int row, int f, int n, int lane) {
+        const int h = lane >> 5;
+        if constexpr (sizeof(T) == 4) {
+            Frag v;
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                const int r = 8 * f + 4 * h + j;
+                v[j] = *reinterpret_cast<const float*>(lds + (row + r) * RB +
+                                                       ((8 * n + ((lane & 31) >> 2)) ^ tile_swz<CPR>(r)) * 16 + 4 * (lane & 3));
+            }
+            return v;
+        } else {
+            const int i = lane & 15, c = 4 * n + 2 * ((lane >> 4) & 1) + ((i & 3) >> 1), r = 16 * f + 4 * h + (i >> 2);
+            const char* p = lds + (row + r) * RB + 8 * (i & 1);
+            union { s16x4 s[2]; Frag f; } u;
+            u.s[0] = lds_read_tr(p + (c ^ tile_swz<CPR>(r)) * 16);
+            u.s[1] = lds_read_tr(p + 8 * RB + (c ^ tile_swz<CPR>(r + 8)) * 16);
+            return u.f;
+        }
+    }
+};
+
+// ROWS rows of an array (element stride between rows) straight into LDS, 16
+// bytes a thread and load, rows past the last and columns past d as zeros
+template <typename T, int DP, int ROWS>
+struct TileLoad {
+    static constexpr int VEC = Mma<T>::VEC, RB = DP * (int)sizeof(T), CPR = RB / 16, N = ROWS * CPR / kAttnThreads;
+    static_assert(N >= 1 && ROWS * CPR % kAttnThreads == 0, "a tile is a whole number of vectors a thread");
+    uint32_t off[N];
+    __device__ __forceinline__ void init(long stride, int d) {
+#pragma unroll
+        for (int i = 0; i < N; i++) {
+            const int v = threadIdx.x + i * kAttnThreads, r = v / CPR, c = v % CPR ^ tile_swz<CPR>(r);
+            // an offset past any buffer's end reads as 0
+            off[i] = c * VEC < d ? (uint32_t)(r * (int)stride * (int)sizeof(T)) + c * 16 : 0x80000000u;
+        }
+    }
+    // the tile's first row at `row`, `left` rows from there on (uniform)
+    __device__ __forceinline__ void issue(char* lds, const T* row, int left, long stride, int d, bool vec, int wave) const {
+        if (vec) {
+            const long bytes = left <= 0 ? 0 : ((left - 1) * stride + d) * (long)sizeof(T);
+            const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc(
+                (void*)row, 0, (int)(bytes < 0x7fffffffL ? bytes : 0x7fffffffL), 0x00027000);
+#pragma unroll
+            for (int i = 0; i < N; i++)
+                __builtin_amdgcn_raw_ptr_buffer_load_lds(
+                    rs, (__attribute__((address_space(3))) void*)(lds + (wave * 64 + i * kAttnThreads) * 16), 16, (int)off[i],
+                    0, 0, 0);
+        } else {
+#pragma unroll
+            for (int i = 0; i < N; i++) {
+                const int v = threadIdx.x + i * kAttnThreads, r = v / CPR, c = v % CPR ^ tile_swz<CPR>(r);
+                *reinterpret_cast<u32x4*>(lds + v * 16) =
+                    r < left ? load_chunk(row + (long)r * stride, c * VEC, d, false) : u32x4{0, 0, 0, 0};
+            }
+        }
+    }
+};
+
+// every load into LDS so far has landed, for all the workgroup's waves
+__device__ __forceinline__ void tiles_landed() {
+    __builtin_amdgcn_s_waitcnt(0x0f70);            // vmcnt(0)
+    __syncthreads();
+}
+
+// The key groups' (or row groups') accumulators of the same columns added
+// into group 0's, 32 rows at a time through `lds` (16 KB a group past the
+// first and column set); all the workgroup's waves call it.
+template <int KG, int WR, int ND>
+__device__ __forceinline__ void join_groups(f32x16 (&o)[ND], float f, char* lds, int wr, int kg, int lane) {
+    float* jo = reinterpret_cast<float*>(lds);
+#pragma unroll
+    for (int i = 0; i < ND; i++) {
+        __syncthreads();
+        if (kg) {
+#pragma unroll
+            for (int e = 0; e < 16; e++) jo[(((kg - 1) * WR + wr) * 16 + e) * 64 + lane] = o[i][e] * f;
+        }
+        __syncthreads();
+        if (!kg) {
+#pragma unroll
+            for (int e = 0; e < 16; e++) {
+                float t = o[i][e] * f;
+#pragma unroll
+                for (int k = 1; k < KG; k++) t += jo[(((k - 1) * WR + wr) * 16 + e) * 64 + lane];
+                o[i][e] = t;
+            }
+        }
+    }
+}
+
 // a row's fragments: value KF f + KF / 2 half of row `row` (global memory)
 template <typename T, int DP>
 __device__ __forceinline__ void load_frags(typename Mma<T>::Frag (&fr)[DP / Mma<T>::KF], const T* row, bool there,

@@ -491,12 +491,16 @@ static int packed_args(const char* who, PackedArgs* a, int dtype) {
     if (rc) return rc;
     if (a->n_seqs < 0 || a->total < 0 || a->total > (1 << 30))
         return fail(RAC_ERR_INVALID_DIM, "%s: n_seqs and total must not be negative, total at most 2^30", who);
-    if (((long)a->total / 128 + a->n_seqs + 2) * a->heads > 2147483647L)
+    if (((long)a->total / 32 + a->n_seqs + 2) * a->heads > 2147483647L)
         return fail(RAC_ERR_INVALID_DIM, "%s: too many sequences and heads", who);
     if (a->sq_t < 0 || a->sq_h < 0 || a->sk_t < 0 || a->sk_h < 0 || a->sv_t < 0 || a->sv_h < 0)
         return fail(RAC_ERR_INVALID_DIM, "%s: strides must not be negative", who);
     const int es = dtype == 0 ? 4 : 2;
-    a->vec = rows_aligned(a->q, es, a->d, a->sq_t, a->sq_h) && rows_aligned(a->k, es, a->d, a->sk_t, a->sk_h) &&
+    // 16 bytes at a time: rows that start on such boundaries, do not overlap
+    // and lie at most 4 MB apart (a tile's offsets are 32-bit)
+    const long near = (4L << 20) / es;
+    a->vec = a->sq_t >= a->d && a->sk_t >= a->d && a->sv_t >= a->d && a->sq_t <= near && a->sk_t <= near &&
+             a->sv_t <= near && (long)a->heads * a->d <= near && rows_aligned(a->q, es, a->d, a->sq_t, a->sq_h) && rows_aligned(a->k, es, a->d, a->sk_t, a->sk_h) &&
              rows_aligned(a->v, es, a->d, a->sv_t, a->sv_h);
     return RAC_OK;
 }

@@ -50,6 +50,12 @@ struct Mma<float> {
     static __device__ __forceinline__ float from_f32(float v) { return v; }
 };
 
+// a transposing read of LDS: 16 lanes bring 4 rows of 16 columns (lane i the
+// four columns from 4 (i % 4) of row i / 4), lane i keeps column i
+__device__ __forceinline__ s16x4 lds_read_tr(const void* p) {
+    return __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)p);
+}
+
 // 16-bit operands: T's bits travel as shorts, the instruction knows the type
 template <typename T, typename V8>
 struct MmaHalf {
@@ -68,12 +74,9 @@ struct MmaHalf {
     static __device__ __forceinline__ Frag load_tr(const T* p, int ld, int f, int lane) {
         const int i = lane & 15;
         const T* r = p + (16 * f + 4 * (lane >> 5) + (i >> 2)) * ld + (lane & 16) + 4 * (i & 3);
-        using lds_t = __attribute__((address_space(3))) s16x4;
-        s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_t*)(r));
-        s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_t*)(r + 8 * ld));
         union { s16x4 s[2]; Frag f; } u;
-        u.s[0] = lo;
-        u.s[1] = hi;
+        u.s[0] = lds_read_tr(r);
+        u.s[1] = lds_read_tr(r + 8 * ld);
         return u.f;
     }
     static __device__ __forceinline__ float to_f32(T v) { return (float)v; }
