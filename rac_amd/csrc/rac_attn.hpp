@@ -7,31 +7,17 @@
 
 namespace rac {
 
+// for the lambdas of the kernels: a call of one would lose what is uniform
+#define ATTN_INLINE __attribute__((always_inline))
+
 constexpr int kAttnThreads = 256, kAttnWaves = 4;
 
-// BN rows of a [total, heads, d] array's head (rows first .. of a sequence of
-// len rows; past it zeros) through registers into LDS rows of LD values
-template <typename T, int DP, int BN>
-struct TileStage {
-    static constexpr int VEC = Mma<T>::VEC, CPR = DP / VEC, N = BN * CPR / kAttnThreads;
-    static_assert(N >= 1 && BN * CPR % kAttnThreads == 0, "a tile is a whole number of vectors a thread");
-    u32x4 r[N];
-    __device__ __forceinline__ void load(const T* base, long stride, int first, int len, int d, bool vec) {
-#pragma unroll
-        for (int i = 0; i < N; i++) {
-            const int v = threadIdx.x + i * kAttnThreads, row = first + v / CPR, c = v % CPR * VEC;
-            r[i] = row < len ? load_chunk(base + (long)row * stride, c, d, vec) : u32x4{0, 0, 0, 0};
-        }
-    }
-    template <int LD>
-    __device__ __forceinline__ void store(T* lds) const {
-#pragma unroll
-        for (int i = 0; i < N; i++) {
-            const int v = threadIdx.x + i * kAttnThreads;
-            *reinterpret_cast<u32x4*>(lds + v / CPR * LD + v % CPR * VEC) = r[i];
-        }
-    }
-};
+// v, as a value of its own: addresses made of it are made where they are used
+// and hold no registers between
+__device__ __forceinline__ int attn_fresh(int v) {
+    asm volatile("" : "+v"(v));
+    return v;
+}
 
 // A tile of rows in LDS: row r's 16-byte vectors lie in it without padding,
 // vector c at place c ^ tile_swz(r), so that both ways of reading a tile, 32
@@ -78,42 +64,76 @@ struct Tile {
     }
 };
 
-// ROWS rows of an array (element stride between rows) straight into LDS, 16
-// bytes a thread and load, rows past the last and columns past d as zeros
-template <typename T, int DP, int ROWS>
+// ROWS rows of an array (element stride between rows) into LDS, 16 bytes a
+// thread and load, rows past the last and columns past d as zeros: issue()
+// before the work on the tile before, commit() behind it.
+// DIRECT: straight into LDS, which spares registers and instructions, else
+// through registers.  Before a transposing read (16-bit types) the compiler
+// waits for every load into LDS, whatever its place, so that a direct load has
+// only the time up to the first of them: enough where the rows come from L2 and
+// the scores stand between, too little where they come from HBM.
+template <typename T, int DP, int ROWS, bool DIRECT = sizeof(T) == 4>
 struct TileLoad {
     static constexpr int VEC = Mma<T>::VEC, RB = DP * (int)sizeof(T), CPR = RB / 16, N = ROWS * CPR / kAttnThreads;
     static_assert(N >= 1 && ROWS * CPR % kAttnThreads == 0, "a tile is a whole number of vectors a thread");
-    uint32_t off[N];
+    // Loads i and i + P of a thread read the same vector of rows whose distance
+    // is uniform: one offset serves them, on bases apart.
+    static constexpr int STEP = kAttnThreads / CPR;        // rows a load of the workgroup covers
+    static constexpr int P = kAttnThreads % CPR ? N : STEP % 16 == 0 ? 1 : STEP % 8 == 0 && N > 1 ? 2 : N;
+    uint32_t off[P];
+    u32x4 r[DIRECT ? 1 : N];
     __device__ __forceinline__ void init(long stride, int d) {
 #pragma unroll
-        for (int i = 0; i < N; i++) {
+        for (int i = 0; i < P; i++) {
             const int v = threadIdx.x + i * kAttnThreads, r = v / CPR, c = v % CPR ^ tile_swz<CPR>(r);
             // an offset past any buffer's end reads as 0
             off[i] = c * VEC < d ? (uint32_t)(r * (int)stride * (int)sizeof(T)) + c * 16 : 0x80000000u;
         }
     }
+    __device__ __forceinline__ void load(char* lds, int i, __amdgpu_buffer_rsrc_t rs, int base, int wave) {
+        if constexpr (DIRECT)
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(
+                rs, (__attribute__((address_space(3))) void*)(lds + (wave * 64 + i * kAttnThreads) * 16), 16, (int)off[i % P],
+                base, 0, 0);
+        else
+            r[i] = __builtin_amdgcn_raw_buffer_load_b128(rs, (int)off[i % P], base, 0);
+    }
     // the tile's first row at `row`, `left` rows from there on (uniform)
-    __device__ __forceinline__ void issue(char* lds, const T* row, int left, long stride, int d, bool vec, int wave) const {
-        if (vec) {
-            const long bytes = left <= 0 ? 0 : ((left - 1) * stride + d) * (long)sizeof(T);
-            const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc(
-                (void*)row, 0, (int)(bytes < 0x7fffffffL ? bytes : 0x7fffffffL), 0x00027000);
+    __device__ __forceinline__ void issue(char* lds, const T* row, int left, long stride, int d, bool vec, int wave) {
+        if (vec && left >= ROWS) {
+            const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc((void*)row, 0, 0x7fffffff, 0x00027000);
 #pragma unroll
-            for (int i = 0; i < N; i++)
-                __builtin_amdgcn_raw_ptr_buffer_load_lds(
-                    rs, (__attribute__((address_space(3))) void*)(lds + (wave * 64 + i * kAttnThreads) * 16), 16, (int)off[i],
-                    0, 0, 0);
-        } else {
+            for (int i = 0; i < N; i++) load(lds, i, rs, i / P * P * STEP * (int)stride * (int)sizeof(T), wave);
+        } else if (vec) {
+            // the buffer ends with the last row
 #pragma unroll
             for (int i = 0; i < N; i++) {
-                const int v = threadIdx.x + i * kAttnThreads, r = v / CPR, c = v % CPR ^ tile_swz<CPR>(r);
-                *reinterpret_cast<u32x4*>(lds + v * 16) =
-                    r < left ? load_chunk(row + (long)r * stride, c * VEC, d, false) : u32x4{0, 0, 0, 0};
+                const int skip = i / P * P * STEP, n = left - skip;
+                const int bytes = n <= 0 ? 0 : ((n - 1) * (int)stride + d) * (int)sizeof(T);
+                load(lds, i, __builtin_amdgcn_make_buffer_rsrc((void*)(row + skip * stride), 0, bytes, 0x00027000), 0, wave);
             }
         }
     }
+    // the same tile's arguments
+    __device__ __forceinline__ void commit(char* lds, const T* row, int left, long stride, int d, bool vec) {
+        if (!vec) {
+            const int tid = attn_fresh(threadIdx.x);
+#pragma unroll 1
+            for (int i = 0; i < N; i++) {
+                const int v = tid + i * kAttnThreads, r = v / CPR, c = v % CPR ^ tile_swz<CPR>(r);
+                *reinterpret_cast<u32x4*>(lds + v * 16) =
+                    r < left ? load_chunk(row + (long)r * stride, c * VEC, d, false) : u32x4{0, 0, 0, 0};
+            }
+        } else if constexpr (!DIRECT) {
+#pragma unroll
+            for (int i = 0; i < N; i++) *reinterpret_cast<u32x4*>(lds + (threadIdx.x + i * kAttnThreads) * 16) = r[i];
+        }
+    }
 };
+
+// keeps a rare, uniform branch one: its body would else be done every time,
+// and its results selected
+__device__ __forceinline__ void attn_branch() { asm volatile(""); }
 
 // every load into LDS so far has landed, for all the workgroup's waves
 __device__ __forceinline__ void tiles_landed() {

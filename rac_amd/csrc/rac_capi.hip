@@ -520,11 +520,11 @@ RAC_EXPORT int rac_packed_attention_dev(const void* q, const void* k, const void
     const int es = dtype == 0 ? 4 : 2;
     a.vec_out = (uintptr_t)out % (4 * es) == 0 && d_head % 4 == 0;
     if (total == 0) return RAC_OK;
-    return check_hip(packed_attention_launch(a, dtype, false, (hipStream_t)stream), "rac_packed_attention_dev launch");
+    return check_hip(packed_fwd_launch(a, dtype, (hipStream_t)stream), "rac_packed_attention_dev launch");
 }
 
 RAC_EXPORT long rac_packed_attention_backward_workspace_bytes(int total, int n_heads) {
-    return total > 0 && n_heads > 0 ? 4L * total * n_heads : 0;
+    return total > 0 && n_heads > 0 ? 8L * total * n_heads : 0;
 }
 
 RAC_EXPORT int rac_packed_attention_backward_dev(const void* q, const void* k, const void* v, const void* out,
@@ -546,8 +546,9 @@ RAC_EXPORT int rac_packed_attention_backward_dev(const void* q, const void* k, c
     a.vec = a.vec && rows_aligned(out, es, d_head, 0, 0) && rows_aligned(grad_out, es, d_head, 0, 0);
     a.vec_out = ((uintptr_t)dq | (uintptr_t)dk | (uintptr_t)dv) % (4 * es) == 0 && d_head % 4 == 0;
     if (total == 0) return RAC_OK;
-    return check_hip(packed_attention_launch(a, dtype, true, (hipStream_t)stream),
-                     "rac_packed_attention_backward_dev launch");
+    hipError_t e = packed_dq_launch(a, dtype, (hipStream_t)stream);
+    if (e == hipSuccess) e = packed_dkv_launch(a, dtype, (hipStream_t)stream);
+    return check_hip(e, "rac_packed_attention_backward_dev launch");
 }
 
 static int tree_args(const char* who, const TreeArgs& a, int dtype) {
@@ -559,8 +560,9 @@ static int tree_args(const char* who, const TreeArgs& a, int dtype) {
         return fail(RAC_ERR_INVALID_DIM, "%s: tokens must be in [1, %d]", who, kTreeMaxTokens);
     if (a.cap < a.tokens || a.cap > 2147483647L - 65536)
         return fail(RAC_ERR_INVALID_DIM, "%s: t_cap must hold the tokens and stay below 2^31 - 65536", who);
-    if ((long)a.heads / a.kv_heads * a.tokens > 65535L * 32)
-        return fail(RAC_ERR_INVALID_DIM, "%s: too many query rows of a key / value head", who);
+    // at most 64 splits of the keys
+    if (64L * (a.batch * (long)a.kv_heads + 8) * ((long)a.heads / a.kv_heads * a.tokens / 32 + 1) > 2147483647L)
+        return fail(RAC_ERR_INVALID_DIM, "%s: too many query rows", who);
     return RAC_OK;
 }
 
@@ -598,7 +600,9 @@ RAC_EXPORT int rac_tree_attention_dev(const void* q, const void* k_cache, const 
     if (batch == 0) return RAC_OK;
     if (!workspace && tree_attention_workspace(a, dtype) > 0) return fail(RAC_ERR_NULL_PTR, "%s: null workspace", who);
     const int es = dtype == 0 ? 4 : 2;
-    a.vec = rows_aligned(q, es, d_head, q_stride_b, q_stride_t, q_stride_h) &&
+    const long near = (4L << 20) / es;
+    a.vec = k_stride_t >= d_head && v_stride_t >= d_head && k_stride_t <= near && v_stride_t <= near &&
+            rows_aligned(q, es, d_head, q_stride_b, q_stride_t, q_stride_h) &&
             rows_aligned(k_cache, es, d_head, k_stride_b, k_stride_h, k_stride_t) &&
             rows_aligned(v_cache, es, d_head, v_stride_b, v_stride_h, v_stride_t);
     a.vec_out = (uintptr_t)out % (4 * es) == 0 && d_head % 4 == 0;

@@ -8,7 +8,8 @@
 //   dx_j = g ([j = token] - p_j) - h p_j (logp_j + entropy).
 // One pass over the logits keeps a running maximum, both sums and a wave's
 // list of its largest values; the sums of a row are fp32 sums of at most 32
-// values a lane at a time.  Logits of -inf have probability 0 and no part in
+// values a lane at a time.  In powers of two: e = 2^(x log2 e - r) with r =
+// m log2 e rounded once, whose rounding is a factor of every e and so of l.  Logits of -inf have probability 0 and no part in
 // the entropy; a row of nothing else has log probabilities of -inf, entropy 0
 // and gradients 0.
 //
@@ -29,18 +30,25 @@ __device__ __forceinline__ uint32_t lp_key(float x) {
     const uint32_t u = __builtin_bit_cast(uint32_t, x + 0.0f);
     return (int32_t)u < 0 ? ~u : u | 0x80000000u;
 }
+// the same of bits that are uniform, on the scalar side
+__device__ __forceinline__ uint32_t lp_key_bits(uint32_t u) {
+    if ((u & 0x7fffffffu) > 0x7f800000u) u = 0xff800000u;
+    if (u == 0x80000000u) u = 0;
+    return (int32_t)u < 0 ? ~u : u | 0x80000000u;
+}
 __device__ __forceinline__ float lp_value(uint32_t k) {
     return __builtin_bit_cast(float, (int32_t)k < 0 ? k & 0x7fffffffu : ~k);
 }
 
 // a row's running statistics
 struct LpStat {
-    float m, l, s;                            // maximum, sum e, sum e z
+    float m, l, s;                            // maximum times log2 e (r), sum e, sum e (x log2 e - r)
 };
+constexpr float kLpLn2 = 0.69314718f;
 __device__ __forceinline__ void lp_join(LpStat& a, float m, float l, float s) {
     const float mt = fmaxf(a.m, m);
     const float da = a.m - mt, db = m - mt;   // NaN where both are -inf: l is 0 there
-    const float fa = a.l == 0.0f ? 0.0f : exp2_hw(da * kLog2e), fb = l == 0.0f ? 0.0f : exp2_hw(db * kLog2e);
+    const float fa = a.l == 0.0f ? 0.0f : exp2_hw(da), fb = l == 0.0f ? 0.0f : exp2_hw(db);
     // sum e (z + d), for a part with nothing in it d may be -inf
     const float sa = fa == 0.0f ? 0.0f : fa * __builtin_fmaf(a.l, da, a.s);
     const float sb = fb == 0.0f ? 0.0f : fb * __builtin_fmaf(l, db, s);
@@ -49,18 +57,44 @@ __device__ __forceinline__ void lp_join(LpStat& a, float m, float l, float s) {
     a.m = mt;
 }
 
+// the wave's lanes joined, the same bits in all
+__device__ __forceinline__ void lp_wave_join(LpStat& r) {
+    const int lane = threadIdx.x & 63;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+        const float m = __shfl_xor(r.m, o), l = __shfl_xor(r.l, o), s = __shfl_xor(r.s, o);
+        // the same order of the two in both lanes
+        LpStat p = {lane & o ? m : r.m, lane & o ? l : r.l, lane & o ? s : r.s};
+        lp_join(p, lane & o ? r.m : m, lane & o ? r.l : l, lane & o ? r.s : s);
+        r = p;
+    }
+}
+
+// the value of the lane below (lane 0 keeps its own)
+__device__ __forceinline__ int lane_below(int v) {
+    return __builtin_amdgcn_update_dpp(v, v, 0x138, 0xf, 0xf, false);        // wave_shr:1
+}
+
 // entry (key, tok) into the wave's list
 __device__ __forceinline__ void lp_insert(uint32_t& lk, int& lt, uint32_t key, int tok, int lane) {
     const int at = __popcll(__ballot(lk > key || (lk == key && lt < tok)));
-    const uint32_t pk = __shfl_up(lk, 1);
-    const int pt = __shfl_up(lt, 1);
-    if (lane == at) {
-        lk = key;
-        lt = tok;
-    } else if (lane > at) {
-        lk = pk;
-        lt = pt;
+    const uint32_t pk = (uint32_t)lane_below((int)lk);
+    const int pt = lane_below(lt);
+    lk = lane == at ? key : lane > at ? pk : lk;
+    lt = lane == at ? tok : lane > at ? pt : lt;
+}
+
+// A threshold that at least `top` of the wave's values exceed (0: none such):
+// just below the top-th largest of the lanes' own maxima.
+__device__ __forceinline__ uint32_t lp_start(uint32_t mine, int top) {
+    int above = 0;
+    for (int i = 0; i < 64; i++) {
+        const uint32_t k = (uint32_t)__builtin_amdgcn_readlane((int)mine, i);
+        above += k > mine || (k == mine && i < (int)(threadIdx.x & 63));
     }
+    const uint64_t at = __ballot(above == top - 1);
+    const uint32_t k = (uint32_t)__builtin_amdgcn_readlane((int)mine, __ffsll((unsigned long long)at) - 1);
+    return k ? k - 1 : 0;
 }
 
 // the lists of the workgroup's waves into the `top` best, rank by rank
@@ -72,11 +106,19 @@ __device__ __forceinline__ void lp_rank(uint32_t lk, int lt, int top, uint32_t (
     __syncthreads();
     if (lane < top) {
         int rank = 0;
+#pragma unroll
         for (int w = 0; w < kLpWaves; w++)
-            for (int i = 0; i < top; i++) {
-                const uint32_t k = sk[w][i];
-                // empty entries alike but for their place
-                rank += k > lk || (k == lk && (st[w][i] < lt || (st[w][i] == lt && 64 * w + i < 64 * wave + lane)));
+            for (int i = 0; i < top; i += 4) {
+                const u32x4 k4 = *reinterpret_cast<const u32x4*>(&sk[w][i]);
+                const u32x4 t4 = *reinterpret_cast<const u32x4*>(&st[w][i]);
+#pragma unroll
+                for (int j = 0; j < 4; j++) {
+                    // empty entries alike but for their place
+                    const uint32_t k = k4[j];
+                    const int t = (int)t4[j];
+                    rank += i + j < top &&
+                            (k > lk || (k == lk && (t < lt || (t == lt && 64 * w + i + j < 64 * wave + lane))));
+                }
             }
         if (rank < top) {
             ok[rank] = lk;
@@ -91,15 +133,17 @@ template <typename T>
 __device__ __forceinline__ void lp_finish(const LogprobArgs& a, long row, const LpStat& r, const uint32_t* ok,
                                           const int* ot) {
     const bool empty = r.m == -__builtin_inff() && r.l == 0.0f;
-    const float ll = __builtin_logf(r.l), lse = empty ? -__builtin_inff() : r.m + ll;
-    auto logp = [&](float x) { return x == -__builtin_inff() && r.l == r.l ? x : x - r.m - ll; };
+    const float ll = __builtin_logf(r.l), lse = empty ? -__builtin_inff() : __builtin_fmaf(r.m, kLpLn2, ll);
+    auto logp = [&](float x) {
+        return x == -__builtin_inff() && r.l == r.l ? x : __builtin_fmaf(x, kLog2e, -r.m) * kLpLn2 - ll;
+    };
     if (threadIdx.x == 0) {
         const long t = a.tok[row];
         float lp = 0.0f;                      // a negative token: none
         if (t >= a.vocab) lp = __builtin_nanf("");
         else if (t >= 0) lp = logp(Mma<T>::to_f32(((const T*)a.x)[row * a.stride + t]));
         a.lp[row] = lp;
-        a.ent[row] = empty ? 0.0f : ll - r.s / r.l;
+        a.ent[row] = empty ? 0.0f : ll - r.s / r.l * kLpLn2;
         if (a.lse) a.lse[row] = lse;
     }
     if ((int)threadIdx.x < a.top) {
@@ -112,8 +156,8 @@ __device__ __forceinline__ void lp_finish(const LogprobArgs& a, long row, const 
 template <typename T, bool TOP>
 __global__ __launch_bounds__(kLpThreads) void logprob_kernel(const LogprobArgs a) {
     constexpr int VEC = Mma<T>::VEC, U = 4;                // U vectors of a thread in flight
-    __shared__ uint32_t sk[TOP ? kLpWaves : 1][kLogprobMaxTop], ok[kLogprobMaxTop];
-    __shared__ int st[TOP ? kLpWaves : 1][kLogprobMaxTop], ot[kLogprobMaxTop];
+    __shared__ __attribute__((aligned(16))) uint32_t sk[TOP ? kLpWaves : 1][kLogprobMaxTop], ok[kLogprobMaxTop];
+    __shared__ __attribute__((aligned(16))) int st[TOP ? kLpWaves : 1][kLogprobMaxTop], ot[kLogprobMaxTop];
     __shared__ float red[kLpWaves][3];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const long row = blockIdx.x;
@@ -127,7 +171,6 @@ __global__ __launch_bounds__(kLpThreads) void logprob_kernel(const LogprobArgs a
     uint32_t lk = 0;                                       // 0: nothing yet
     int lt = 0x7fffffff;
     uint32_t thr = 0;
-    bool nan = false;
     for (long b = v0; b < v1; b += U * kLpThreads) {
         float f[U][VEC];
 #pragma unroll
@@ -150,35 +193,44 @@ __global__ __launch_bounds__(kLpThreads) void logprob_kernel(const LogprobArgs a
 #pragma unroll
             for (int e = 0; e < VEC; e++) {
                 mx = fmaxf(mx, f[u][e]);
-                nan |= f[u][e] != f[u][e];
             }
         if constexpr (TOP) {
             if (__any(lp_key(mx) > thr)) {
+                // keys of places past the row are never offered, but count as
+                // -inf here, which at worst is too low a threshold
+                if (b == v0) thr = lp_start(lp_key(mx), a.top);
 #pragma unroll
                 for (int u = 0; u < U; u++) {
                     float um = f[u][0];
 #pragma unroll
                     for (int e = 1; e < VEC; e++) um = fmaxf(um, f[u][e]);
                     const long v = b + u * kLpThreads + tid, c = v * VEC - off;
-                    uint64_t cand = __ballot(v < v1 && lp_key(um) > thr);
-                    for (; cand; cand &= cand - 1) {
+                    const uint32_t uk = v < v1 ? lp_key(um) : 0;
+                    for (uint64_t cand = __ballot(uk > thr); cand;) {
                         const int src = __ffsll((unsigned long long)cand) - 1;
 #pragma unroll
                         for (int e = 0; e < VEC; e++) {
-                            const uint32_t key = __builtin_amdgcn_readlane(lp_key(f[u][e]), src);
-                            const int tok = __builtin_amdgcn_readlane((int)(c + e), src);
-                            if (key > thr && tok >= 0 && tok < a.vocab) {
-                                lp_insert(lk, lt, key, tok, lane);
-                                thr = __builtin_amdgcn_readlane(lk, a.top - 1);
+                            const float fe = f[u][e];
+                            const uint32_t key = lp_key_bits(__builtin_amdgcn_readlane(__builtin_bit_cast(int, fe), src));
+                            if (key > thr) {
+                                const int tok = __builtin_amdgcn_readlane((int)(c + e), src);
+                                if (tok >= 0 && tok < a.vocab) {
+                                    lp_insert(lk, lt, key, tok, lane);
+                                    const uint32_t last = __builtin_amdgcn_readlane(lk, a.top - 1);
+                                    if (last > thr) thr = last;
+                                }
                             }
                         }
+                        // the lanes behind that still have one
+                        cand = src == 63 ? 0 : __ballot(uk > thr) & (~0ull << (src + 1));
                     }
                 }
             }
         }
+        mx *= kLog2e;
         if (mx > r.m) {
             const float d = r.m - mx;
-            const float g = exp2_hw(d * kLog2e);
+            const float g = exp2_hw(d);
             r.s = g == 0.0f ? 0.0f : g * __builtin_fmaf(r.l, d, r.s);
             r.l *= g;
             r.m = mx;
@@ -189,23 +241,15 @@ __global__ __launch_bounds__(kLpThreads) void logprob_kernel(const LogprobArgs a
         for (int u = 0; u < U; u++)
 #pragma unroll
             for (int e = 0; e < VEC; e++) {
-                const float z = fmaxf(f[u][e] - mu, -1000.0f);     // -inf: e is 0, and e z too
-                const float p = exp2_hw(z * kLog2e);
+                const float z = __builtin_fmaf(f[u][e], kLog2e, -mu), p = exp2_hw(z);
                 bl += p;
-                bs = __builtin_fmaf(p, z, bs);
+                bs = __builtin_fmaf(p, fmaxf(z, -1e4f), bs);       // p is 0 there, z may be -inf
             }
         r.l += bl;
         r.s += bs;
     }
-    if (nan || r.m == __builtin_inff()) r.l = r.s = __builtin_nanf("");
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-        const float m = __shfl_xor(r.m, o), l = __shfl_xor(r.l, o), s = __shfl_xor(r.s, o);
-        // the same order of the two in both lanes
-        LpStat p = {lane & o ? m : r.m, lane & o ? l : r.l, lane & o ? s : r.s};
-        lp_join(p, lane & o ? r.m : m, lane & o ? r.l : l, lane & o ? r.s : s);
-        r = p;
-    }
+    // NaN came through l; infinity less itself did too
+    lp_wave_join(r);
     if (lane == 0) {
         red[wave][0] = r.m;
         red[wave][1] = r.l;
@@ -235,27 +279,39 @@ __global__ __launch_bounds__(kLpThreads) void logprob_kernel(const LogprobArgs a
 // The splits of a row joined.
 template <typename T, bool TOP>
 __global__ __launch_bounds__(kLpThreads) void logprob_join_kernel(const LogprobArgs a) {
-    __shared__ uint32_t sk[TOP ? kLpWaves : 1][kLogprobMaxTop], ok[kLogprobMaxTop];
-    __shared__ int st[TOP ? kLpWaves : 1][kLogprobMaxTop], ot[kLogprobMaxTop];
+    __shared__ __attribute__((aligned(16))) uint32_t sk[TOP ? kLpWaves : 1][kLogprobMaxTop], ok[kLogprobMaxTop];
+    __shared__ __attribute__((aligned(16))) int st[TOP ? kLpWaves : 1][kLogprobMaxTop], ot[kLogprobMaxTop];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const long row = blockIdx.x;
     const int width = 3 + 2 * a.top;
     const float* p = a.part + row * a.splits * width;
-    LpStat r = {p[0], p[1], p[2]};
-    for (int s = 1; s < a.splits; s++) lp_join(r, p[s * width], p[s * width + 1], p[s * width + 2]);
+    LpStat r = {-__builtin_inff(), 0.0f, 0.0f};
+    for (int s = lane; s < a.splits; s += 64) lp_join(r, p[s * width], p[s * width + 1], p[s * width + 2]);
+    lp_wave_join(r);
     if constexpr (TOP) {
-        uint32_t lk = 0;
-        int lt = 0x7fffffff;
-        for (int s = wave; s < a.splits; s += kLpWaves) {
-            const uint32_t* pk = reinterpret_cast<const uint32_t*>(p + s * width + 3);
-            const uint32_t mk = lane < a.top ? pk[lane] : 0;
-            const int mt = lane < a.top ? (int)pk[a.top + lane] : 0x7fffffff;
+        // the wave's first list as it stands; the next one's loads ahead of its turn
+        const uint32_t* list = reinterpret_cast<const uint32_t*>(p) + 3;
+        auto load = [&](int s, uint32_t& k, int& t) {
+            const bool there = s < a.splits && lane < a.top;
+            k = there ? list[s * width + lane] : 0;
+            t = there ? (int)list[s * width + a.top + lane] : 0x7fffffff;
+        };
+        uint32_t lk, mk;
+        int lt, mt;
+        load(wave, lk, lt);
+        load(wave + kLpWaves, mk, mt);
+        for (int s = wave + kLpWaves; s < a.splits; s += kLpWaves) {
+            uint32_t nk;
+            int nt;
+            load(s + kLpWaves, nk, nt);
             for (int i = 0; i < a.top; i++) {
                 const uint32_t key = __builtin_amdgcn_readlane(mk, i);
                 // splits come in token order: an equal key's token is higher
                 if (key <= __builtin_amdgcn_readlane(lk, a.top - 1)) break;
                 lp_insert(lk, lt, key, __builtin_amdgcn_readlane(mt, i), lane);
             }
+            mk = nk;
+            mt = nt;
         }
         lp_rank(lk, lt, a.top, sk, st, ok, ot);
     }

@@ -7,9 +7,10 @@
 // 32x32x2 (4 values, value j of the two halves being the two k of instruction
 // j).  The accumulator of a product has column l % 32 and, in register 4 b + j,
 // row 8 b + 4 h + j: KF k of a following product are KF / 2 neighbouring
-// registers, so an accumulator turns into that product's right operand without
-// leaving its lane, as long as the left operand's fragments hold their k in the
-// same order (load_tr).
+// registers, so an accumulator turns into that product's right operand (pack)
+// without leaving its lane, as long as the left operand's fragments hold their k
+// in the same order: of every KF the half h the rows 4 h + j, and for the 16-bit
+// types 8 + 4 h + j, j = 0 .. 3 (Tile::cols).
 #pragma once
 #include <hip/hip_runtime.h>
 #include <stdint.h>
@@ -41,11 +42,6 @@ struct Mma<float> {
     static __device__ __forceinline__ Frag pack(const f32x16& c, int f) {
         return Frag{c[4 * f], c[4 * f + 1], c[4 * f + 2], c[4 * f + 3]};
     }
-    // rows 8 f + 4 h + j of the 32 at p, column l % 32 (p points at row 0, column 0)
-    static __device__ __forceinline__ Frag load_tr(const float* p, int ld, int f, int lane) {
-        const float* r = p + (8 * f + 4 * (lane >> 5)) * ld + (lane & 31);
-        return Frag{r[0], r[ld], r[2 * ld], r[3 * ld]};
-    }
     static __device__ __forceinline__ float to_f32(float v) { return v; }
     static __device__ __forceinline__ float from_f32(float v) { return v; }
 };
@@ -67,17 +63,6 @@ struct MmaHalf {
 #pragma unroll
         for (int j = 0; j < 8; j++) r[j] = (T)c[8 * f + j];      // to nearest even
         return r;
-    }
-    // rows 16 f + {4 h + j, 8 + 4 h + j} of the 32 at p, column l % 32: two
-    // transposing reads, in which 16 lanes bring 4 rows of 16 columns (lane i
-    // the four columns from 4 (i % 4) of row i / 4) and lane i keeps column i
-    static __device__ __forceinline__ Frag load_tr(const T* p, int ld, int f, int lane) {
-        const int i = lane & 15;
-        const T* r = p + (16 * f + 4 * (lane >> 5) + (i >> 2)) * ld + (lane & 16) + 4 * (i & 3);
-        union { s16x4 s[2]; Frag f; } u;
-        u.s[0] = lds_read_tr(r);
-        u.s[1] = lds_read_tr(r + 8 * ld);
-        return u.f;
     }
     static __device__ __forceinline__ float to_f32(T v) { return (float)v; }
     static __device__ __forceinline__ T from_f32(float v) { return (T)v; }

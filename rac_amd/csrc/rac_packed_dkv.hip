@@ -1,0 +1,221 @@
+// rac_packed_dkv.hip — packed causal attention, the gradients of k and v.
+#include "rac_packed.hpp"
+
+namespace rac {
+
+// WHICH: 1 dv, 2 dk, 3 both (d past 128 in fp32 has no registers for both)
+template <typename T, int DP, int WR, int WHICH>
+__global__ __launch_bounds__(kPkThreads, DP * sizeof(T) <= 128 ? 2 : 1) void packed_dkv_kernel(const PackedArgs a) {
+    using M = Mma<T>;
+    using Frag = typename M::Frag;
+    using S = PackedShape<T, DP, WR>;
+    using TL = Tile<T, DP>;
+    constexpr int KG = S::KG, BQ = S::BN, TILE = S::TILE, ND = S::ND, NF = S::NF, NS = S::NS, FS = S::FS;
+    constexpr bool WV = WHICH & 1, WK = WHICH & 2;
+    __shared__ __attribute__((aligned(16))) char qa[S::BYTES], ga[S::BYTES], qb[S::BYTES], gb[S::BYTES];
+    __shared__ __attribute__((aligned(16))) float sa[2 * TILE], sb[2 * TILE];       // log2 sums and D
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), half = lane >> 5;
+    const int wr = wave % WR, kg = wave / WR;
+    int g, tile;
+    packed_block(a.kv_heads, g, tile);
+    const PackedSeg seg = packed_tile(a.cu, a.n_seqs, a.total, tile, S::ROWS, true);
+    if (seg.kind == 0) return;
+    T* dk = (T*)a.dk;
+    T* dv = (T*)a.dv;
+    if (seg.kind == 2) {
+        const int rows = min(S::ROWS, seg.len - seg.row0);
+        if (a.zero_rest) {
+            if (WK) packed_zero(dk, seg.start + seg.row0, rows, a.kv_heads, g, a.d);
+            if (WV) packed_zero(dv, seg.start + seg.row0, rows, a.kv_heads, g, a.d);
+        }
+        return;
+    }
+    const int k0 = seg.row0, kw = k0 + 32 * wr, key = kw + (lane & 31);
+    const int rep = a.heads / a.kv_heads;
+    const bool there = key < seg.len;
+    const long row = seg.start + key;
+    // steps: the tiles of queries from the diagonal on, for one head of the group after the other
+    const int t0 = k0 / TILE, per = (seg.len + TILE - 1) / TILE - t0, steps = per * rep;
+    const T* const Q = (const T*)a.q + (long)seg.start * a.sq_t + (long)g * rep * a.sq_h;
+    const T* const G = (const T*)a.grad + ((long)seg.start * a.heads + (long)g * rep) * a.d;
+    // direct also in 16 bits: 6 bf16 documents of 8192 rows (32/8 heads of 128)
+    // 795 us, through registers 870
+    TileLoad<T, DP, TILE, true> lq, lg;
+    lq.init(a.sq_t, a.d);
+    lg.init((long)a.heads * a.d, a.d);
+    int ih = 0, it = t0;                                  // head and tile of the next issue
+    const int slot = threadIdx.x;                         // a thread's value of a tile's log sums and D
+    float stat_next = 0.0f;
+    auto issue = [&](char* qd, char* gd) ATTN_INLINE {
+        const int first = it * TILE, left = seg.len - first;
+        lq.issue(qd, Q + (long)ih * a.sq_h + (long)first * a.sq_t, left, a.sq_t, a.d, a.vec, wave);
+        lg.issue(gd, G + (long)ih * a.d + (long)first * a.heads * a.d, left, (long)a.heads * a.d, a.d, a.vec, wave);
+        if (slot < 2 * TILE) {
+            const float* base = a.stats + 2 * ((long)(g * rep + ih) * a.total + seg.start + first);
+            // rows past the sequence: 0, next to zeros of do no matter
+            stat_next = slot < 2 * left ? base[slot] : 0.0f;
+        }
+    };
+    // behind the work on the tile before
+    auto commit = [&](char* qd, char* gd, float* st) ATTN_INLINE {
+        if (slot < 2 * TILE) st[slot] = stat_next;
+        const int first = it * TILE, left = seg.len - first;
+        lq.commit(qd, Q + (long)ih * a.sq_h + (long)first * a.sq_t, left, a.sq_t, a.d, a.vec);
+        lg.commit(gd, G + (long)ih * a.d + (long)first * a.heads * a.d, left, (long)a.heads * a.d, a.d, a.vec);
+        if (++it == t0 + per) {
+            it = t0;
+            ih++;
+        }
+    };
+    issue(qa, ga);
+    Frag kf[NF], vf[WK ? NF : 1];
+    load_frags<T, DP>(kf, (const T*)a.k + row * a.sk_t + (long)g * a.sk_h, there, a.d, half, a.vec);
+    if constexpr (WK) load_frags<T, DP>(vf, (const T*)a.v + row * a.sv_t + (long)g * a.sv_h, there, a.d, half, a.vec);
+    const float c = a.scale * kLog2e;
+    f32x16 ak[WK ? ND : 1], av[WV ? ND : 1];
+#pragma unroll
+    for (int n = 0; n < ND; n++) {
+        if constexpr (WK) ak[n] = zero16();
+        if constexpr (WV) av[n] = zero16();
+    }
+    int ct = t0;                                          // tile of this step
+    auto work = [&](const char* qs, const char* gs, const float* ss) ATTN_INLINE {
+        const int first = ct * TILE + kg * BQ, row0 = kg * BQ;
+        if (++ct == t0 + per) ct = t0;
+        auto scores = [&](int u, f32x16& s, f32x16& dp) ATTN_INLINE {
+            s = zero16();
+            dp = zero16();
+#pragma unroll
+            for (int f = 0; f < NF; f++) {
+                s = M::mma(TL::rows(qs, row0 + 32 * u, f, lane), kf[f], s);
+                if constexpr (WK) dp = M::mma(TL::rows(gs, row0 + 32 * u, f, lane), vf[f], dp);
+            }
+        };
+        auto weights = [&](int u, f32x16& s, f32x16& dp) ATTN_INLINE {
+#pragma unroll
+            for (int b = 0; b < 4; b++) {
+                const f32x4* st = reinterpret_cast<const f32x4*>(ss + 2 * (row0 + 32 * u + 8 * b + 4 * half));
+                const f32x4 st0 = st[0], st1 = st[1];
+                const float le[4] = {st0[0], st0[2], st1[0], st1[2]}, de[4] = {st0[1], st0[3], st1[1], st1[3]};
+#pragma unroll
+                for (int j = 0; j < 4; j++) {
+                    const int i = 4 * b + j;
+                    s[i] = exp2_hw(__builtin_fmaf(s[i], c, -le[j]));
+                    if constexpr (WK) dp[i] = s[i] * (dp[i] - de[j]);
+                }
+            }
+        };
+        auto sums = [&](int u, const f32x16& s, const f32x16& dp) ATTN_INLINE {
+#pragma unroll
+            for (int f = 0; f < FS; f++) {
+                Frag pf, df;
+                if constexpr (WV) pf = M::pack(s, f);
+                if constexpr (WK) df = M::pack(dp, f);
+#pragma unroll
+                for (int n = 0; n < ND; n++) {
+                    if constexpr (WV) av[n] = M::mma(TL::cols(gs, row0 + 32 * u, f, n, lane), pf, av[n]);
+                    if constexpr (WK) ak[n] = M::mma(TL::cols(qs, row0 + 32 * u, f, n, lane), df, ak[n]);
+                }
+            }
+        };
+        if (first >= kw + 31) {
+            // every query sees every key of the wave
+            f32x16 s[NS], dp[NS];
+#pragma unroll
+            for (int u = 0; u < NS; u++) scores(u, s[u], dp[u]);
+#pragma unroll
+            for (int u = 0; u < NS; u++) {
+                weights(u, s[u], dp[u]);
+                sums(u, s[u], dp[u]);
+            }
+            return;
+        }
+#pragma unroll 1
+        for (int u = 0; u < NS; u++) {
+            const int q0 = first + 32 * u;
+            if (q0 + 31 < kw || q0 >= seg.len) continue;     // before the wave's keys, or past the sequence
+            f32x16 s, dp;
+            scores(u, s, dp);
+            weights(u, s, dp);
+#pragma unroll
+            for (int i = 0; i < 16; i++)
+                if (q0 + 8 * (i / 4) + 4 * half + i % 4 < key) {
+                    s[i] = 0.0f;
+                    if constexpr (WK) dp[i] = 0.0f;
+                }
+            sums(u, s, dp);
+        }
+    };
+    auto step = [&](int st, const char* qs, const char* gs, const float* ss, char* qn, char* gn, float* sn) ATTN_INLINE {
+        tiles_landed();
+        if (st + 1 < steps) issue(qn, gn);
+        work(qs, gs, ss);
+        if (st + 1 < steps) commit(qn, gn, sn);
+    };
+    commit(qa, ga, sa);
+    for (int st = 0; st < steps; st += 2) {
+        step(st, qa, ga, sa, qb, gb, sb);
+        if (st + 1 < steps) step(st + 1, qb, gb, sb, qa, ga, sa);
+    }
+    if constexpr (KG > 1) {
+        if constexpr (WK) join_groups<KG, WR, ND>(ak, 1.0f, qa, wr, kg, lane);
+        if constexpr (WV) join_groups<KG, WR, ND>(av, 1.0f, qa, wr, kg, lane);
+        if (kg) return;
+    }
+    bool bad = false;
+    if constexpr (WK) bad |= not_finite(ak);
+    if constexpr (WV) bad |= not_finite(av);
+    uint64_t again = __ballot(bad && there);
+    again = (again | again >> 32) & 0xffffffffull;
+    if (there && !(again >> (lane & 31) & 1)) {
+        const long at = (row * a.kv_heads + g) * a.d;
+        if constexpr (WK) attn_store<T, ND>(dk + at, ak, a.scale, a.d, half, a.vec_out);
+        if constexpr (WV) attn_store<T, ND>(dv + at, av, 1.0f, a.d, half, a.vec_out);
+    }
+    for (; again; again &= again - 1) {
+        const int kr = kw + __ffsll((unsigned long long)again) - 1, from = kr, n = seg.len - from;
+        const long at = ((long)(seg.start + kr) * a.kv_heads + g) * a.d;
+        const T* kk = (const T*)a.k + (long)(seg.start + kr) * a.sk_t + (long)g * a.sk_h;
+        const T* vv = (const T*)a.v + (long)(seg.start + kr) * a.sv_t + (long)g * a.sv_h;
+        // queries from .. of head 0 of the group, then of head 1, ...
+        auto qrow = [&](int i) { return Q + (long)(i / n) * a.sq_h + (long)(from + i % n) * a.sq_t; };
+        auto grow = [&](int i) { return G + ((long)(from + i % n) * a.heads + i / n) * a.d; };
+        auto stats_of = [&](int i) { return a.stats + 2 * ((long)(g * rep + i / n) * a.total + seg.start + from + i % n); };
+        auto prob = [&](int i) { return exp2_hw(__builtin_fmaf(row_dot(qrow(i), kk, a.d), c, -*stats_of(i))); };
+        if constexpr (WV) attn_again<T, DP>(dv + at, 1.0f, a.d, 0, n * rep, prob, grow);
+        if constexpr (WK)
+            attn_again<T, DP>(dk + at, a.scale, a.d, 0, n * rep,
+                                [&](int i) { return prob(i) * (row_dot(grow(i), vv, a.d) - stats_of(i)[1]); }, qrow);
+    }
+}
+
+// ── launch ──────────────────────────────────────────────────────────────
+
+namespace {
+struct Launch {
+    const PackedArgs& a;
+    hipStream_t s;
+    template <typename T, int DP, int WR>
+    void sets() const {
+        const dim3 grid((unsigned)(packed_tiles(a, 32 * WR) * a.kv_heads)), t(kPkThreads);
+        if constexpr (DP * sizeof(T) > 512) {
+            hipLaunchKernelGGL((packed_dkv_kernel<T, DP, WR, 1>), grid, t, 0, s, a);
+            hipLaunchKernelGGL((packed_dkv_kernel<T, DP, WR, 2>), grid, t, 0, s, a);
+        } else {
+            hipLaunchKernelGGL((packed_dkv_kernel<T, DP, WR, 3>), grid, t, 0, s, a);
+        }
+    }
+    template <typename T, int DP>
+    void run() const {
+        if (packed_few(a, a.kv_heads)) sets<T, DP, packed_few_sets<T, DP>()>();
+        else sets<T, DP, 4>();
+    }
+};
+}  // namespace
+
+hipError_t packed_dkv_launch(const PackedArgs& a, int dtype, hipStream_t s) {
+    packed_by_type(dtype, a.d, Launch{a, s});
+    return hipGetLastError();
+}
+
+}  // namespace rac

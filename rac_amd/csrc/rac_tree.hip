@@ -23,34 +23,41 @@ namespace rac {
 constexpr int kTreeThreads = kAttnThreads;
 constexpr int kTreeWords = kTreeMaxTokens / 32 + 1;       // one more, always 0, for reads of 32 bits at any place
 
-// keys a wave takes at a time, and those of a tile: one such set for each of
-// the workgroup's key groups
-constexpr int tree_bn(int es, int wr) { return es == 2 && wr == kAttnWaves ? 64 : 32; }
-constexpr int tree_tile(int es, int wr) { return tree_bn(es, wr) * (kAttnWaves / wr); }
+// A workgroup's four waves are WR sets of 32 rows times KG = 4 / WR groups that
+// take different keys of a tile: BN a wave.
+constexpr int tree_bn(int es, int dp, int wr) { return es == 2 && wr == kAttnWaves && dp <= 128 ? 64 : 32; }
+constexpr int tree_tile(int es, int dp, int wr) { return tree_bn(es, dp, wr) * (kAttnWaves / wr); }
 
 // the tiles that split s of `splits` takes out of `tiles`: `per` from s per on
 __device__ __forceinline__ int tree_per(int tiles, int splits) { return (tiles + splits - 1) / splits; }
+
+// part: unnormalised outputs [batch, kv_heads, splits, rows, d], then their
+// maxima and sums [.., rows, 2] from here on
+__host__ __device__ inline long tree_stats(const TreeArgs& a) {
+    return (long)a.batch * a.splits * a.heads * a.tokens * a.d;
+}
 
 template <typename T, int DP, int WR>
 __global__ __launch_bounds__(kTreeThreads, DP * sizeof(T) <= 256 ? 2 : 1) void tree_kernel(const TreeArgs a) {
     using M = Mma<T>;
     using Frag = typename M::Frag;
-    constexpr int KF = M::KF, NF = DP / KF, ND = DP / 32, LD = DP + M::VEC;
-    constexpr int BN = tree_bn(sizeof(T), WR), NS = BN / 32;
-    constexpr int KG = kAttnWaves / WR, TILE = BN * KG;
-    // the waves' outputs are joined where the tiles were
-    constexpr int TILES = 2 * TILE * LD * (int)sizeof(T), JOIN = KG > 1 ? (KG - 1) * WR * 64 * 16 * 4 : 0;
-    __shared__ __attribute__((aligned(16))) char lds[TILES > JOIN ? TILES : JOIN];
+    using TL = Tile<T, DP>;
+    constexpr int NF = DP / M::KF, ND = DP / 32, FS = 32 / M::KF;
+    constexpr int KG = kAttnWaves / WR, BN = tree_bn(sizeof(T), DP, WR), NS = BN / 32, TILE = BN * KG;
+    constexpr int BYTES = TILE * DP * (int)sizeof(T);
+    __shared__ __attribute__((aligned(16))) char ka[BYTES], va[BYTES], kb[BYTES], vb[BYTES];
     __shared__ uint32_t anc[kTreeMaxTokens][kTreeWords];
     __shared__ int up[2][kTreeMaxTokens];
     __shared__ float sm[kAttnWaves][32], sl[kAttnWaves][32];
-    T* const sk = (T*)lds;
-    T* const sv = sk + TILE * LD;
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, half = lane >> 5;
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), half = lane >> 5;
     const int wr = wave % WR, kg = wave / WR;
     const int rep = a.heads / a.kv_heads, rows = rep * a.tokens;
-    const int split = blockIdx.x, rb = blockIdx.y, b = blockIdx.z / a.kv_heads, g = blockIdx.z % a.kv_heads;
-    const int r = (rb * WR + wr) * 32 + (lane & 31);                    // the lane's row
+    // workgroup L runs on XCD L % 8: the row blocks over the same keys follow
+    // each other on one XCD and share its L2
+    const int nb = (rows + 32 * WR - 1) / (32 * WR), i8 = blockIdx.x / 8, rb = i8 % nb, unit = i8 / nb * 8 + blockIdx.x % 8;
+    const int split = unit % a.splits, bg = unit / a.splits, b = bg / a.kv_heads, g = bg % a.kv_heads;
+    if (b >= a.batch) return;
+    const int rw = (rb * WR + wr) * 32, r = rw + (lane & 31);           // the wave's first row, the lane's
     const bool there = r < rows;
     const int tok = there ? r / rep : 0, head = g * rep + (there ? r % rep : 0);
     const int len = a.len[b];
@@ -69,14 +76,30 @@ __global__ __launch_bounds__(kTreeThreads, DP * sizeof(T) <= 256 ? 2 : 1) void t
     const T* K = (const T*)a.k + (long)b * a.sk_b + (long)g * a.sk_g;
     const T* V = (const T*)a.v + (long)b * a.sv_b + (long)g * a.sv_g;
     const T* qrow = (const T*)a.q + (long)b * a.sq_b + (long)tok * a.sq_t + (long)head * a.sq_h;
-    TileStage<T, DP, TILE> rk, rv;
-    rk.load(K, a.sk_t, j0 * TILE, n, a.d, a.vec);
-    rv.load(V, a.sv_t, j0 * TILE, n, a.d, a.vec);
+    // 16 bits through registers: 16 bf16 caches of up to 8001 positions, 64 drafts
+    // each (32/8 heads of 128), 167 us, direct 236
+    TileLoad<T, DP, TILE> lk, lv;
+    lk.init(a.sk_t, a.d);
+    lv.init(a.sv_t, a.d);
+    auto issue = [&](int j, char* kd, char* vd) ATTN_INLINE {
+        lk.issue(kd, K + (long)j * TILE * a.sk_t, n - j * TILE, a.sk_t, a.d, a.vec, wave);
+        lv.issue(vd, V + (long)j * TILE * a.sv_t, n - j * TILE, a.sv_t, a.d, a.vec, wave);
+    };
+    auto commit = [&](int j, char* kd, char* vd) ATTN_INLINE {
+        lk.commit(kd, K + (long)j * TILE * a.sk_t, n - j * TILE, a.sk_t, a.d, a.vec);
+        lv.commit(vd, V + (long)j * TILE * a.sv_t, n - j * TILE, a.sv_t, a.d, a.vec);
+    };
+    // a workgroup begins within its tiles at a place of its own and goes round:
+    // caches whose sequences lie a power of two apart would else be walked in
+    // step, all on the same memory channels at a time
+    const int cnt = j1 - j0, turn = (7 * bg + 3 * split) % cnt;
+    auto tile_of = [&](int i) ATTN_INLINE { return j0 + (i + turn < cnt ? i + turn : i + turn - cnt); };
+    issue(tile_of(0), ka, va);
     Frag qf[NF];
     load_frags<T, DP>(qf, qrow, there, a.d, half, a.vec);
-    const bool tail = j1 * TILE > len;                   // the split holds drafted tokens
-    if (tail) {
-        // paths to the root, a step that doubles what is known at a time
+    if (j1 * TILE > len) {
+        // the split holds drafted tokens: their paths to the root, in steps
+        // that double what is known
         int p = -1;
         if (tid < a.tokens) {
             p = a.parents[(long)b * a.parents_b + tid];
@@ -86,16 +109,17 @@ __global__ __launch_bounds__(kTreeThreads, DP * sizeof(T) <= 256 ? 2 : 1) void t
             for (int w = 0; w < kTreeWords; w++) anc[tid][w] = w == tid / 32 ? 1u << (tid & 31) : 0u;
         }
         for (int hop = 1, cur = 0; hop < a.tokens; hop *= 2, cur ^= 1) {
-            __syncthreads();
+            if (!__syncthreads_or(p >= 0)) break;          // every path known
             uint32_t m[kTreeWords];
-            if (tid < a.tokens && p >= 0) {
+            const bool had = p >= 0;
+            if (had) {
 #pragma unroll
                 for (int w = 0; w < kTreeWords; w++) m[w] = anc[tid][w] | anc[p][w];
                 p = up[cur][p];
             }
             __syncthreads();
             if (tid < a.tokens) {
-                if (up[cur][tid] >= 0) {
+                if (had) {
 #pragma unroll
                     for (int w = 0; w < kTreeWords; w++) anc[tid][w] = m[w];
                 }
@@ -109,7 +133,7 @@ __global__ __launch_bounds__(kTreeThreads, DP * sizeof(T) <= 256 ? 2 : 1) void t
     for (int i = 0; i < ND; i++) o[i] = zero16();
     float m = -__builtin_inff(), l = 0.0f;
     // bits of positions len + u .. + 31 that the row sees, ones before the drafts
-    auto seen = [&](int u) -> uint32_t {
+    auto seen = [&](int u) ATTN_INLINE -> uint32_t {
         if (u >= a.tokens) return 0u;
         if (u <= -32) return ~0u;
         const uint32_t* w = anc[tok];
@@ -117,29 +141,18 @@ __global__ __launch_bounds__(kTreeThreads, DP * sizeof(T) <= 256 ? 2 : 1) void t
         const uint64_t two = w[u >> 5] | (uint64_t)w[(u >> 5) + 1] << 32;
         return (uint32_t)(two >> (u & 31));
     };
-    for (int j = j0; j < j1; j++) {
-        __syncthreads();
-        rk.template store<LD>(sk);
-        rv.template store<LD>(sv);
-        __syncthreads();
-        if (j + 1 < j1) {
-            rk.load(K, a.sk_t, (j + 1) * TILE, n, a.d, a.vec);
-            rv.load(V, a.sv_t, (j + 1) * TILE, n, a.d, a.vec);
-        }
-        const int first = j * TILE + kg * BN;             // the wave's keys
-        if (first >= n) continue;
-        const T* ks = sk + kg * BN * LD;
-        const T* vs = sv + kg * BN * LD;
+    auto work = [&](int i, const char* ks, const char* vs) ATTN_INLINE {
+        const int first = tile_of(i) * TILE + kg * BN;    // the wave's keys
+        if (first >= n || rw >= rows) return;
         f32x16 s[NS];
 #pragma unroll
-        for (int u = 0; u < NS; u++) {
-            s[u] = zero16();
+        for (int u = 0; u < NS; u++) s[u] = zero16();
 #pragma unroll
-            for (int f = 0; f < NF; f++)
-                s[u] = M::mma(*reinterpret_cast<const Frag*>(ks + (32 * u + (lane & 31)) * LD + f * KF +
-                                                             half * (KF / 2)), qf[f], s[u]);
-        }
+        for (int f = 0; f < NF; f++)
+#pragma unroll
+            for (int u = 0; u < NS; u++) s[u] = M::mma(TL::rows(ks, kg * BN + 32 * u, f, lane), qf[f], s[u]);
         if (first + BN > len) {
+            attn_branch();
 #pragma unroll
             for (int u = 0; u < NS; u++) {
                 const uint32_t bits = seen(first + 32 * u - len);
@@ -153,10 +166,20 @@ __global__ __launch_bounds__(kTreeThreads, DP * sizeof(T) <= 256 ? 2 : 1) void t
         for (int u = 0; u < NS; u++)
 #pragma unroll
             for (int i = 0; i < 16; i++) mx = fmaxf(mx, s[u][i]);
-        mx = fmaxf(m, half_max(mx) * c);
-        const float mu = mx == -__builtin_inff() ? 0.0f : mx;
-        const float al = exp2_hw(m - mu);
-        m = mx;
+        mx = half_max(mx) * c;
+        // the maximum that exponents refer to may lag behind by a factor of 2^8
+        if (__any(mx > m + 8.0f)) {
+            const float mt = fmaxf(m, mx);
+            // nothing but -inf so far: exponents of -inf, not NaN
+            const float al = exp2_hw(m - (mt == -__builtin_inff() ? 0.0f : mt));
+            m = mt;
+            l *= al;
+#pragma unroll
+            for (int i = 0; i < ND; i++)
+#pragma unroll
+                for (int e = 0; e < 16; e++) o[i][e] *= al;
+        }
+        const float mu = m == -__builtin_inff() ? 0.0f : m;
         float ls = 0.0f;
 #pragma unroll
         for (int u = 0; u < NS; u++)
@@ -165,25 +188,29 @@ __global__ __launch_bounds__(kTreeThreads, DP * sizeof(T) <= 256 ? 2 : 1) void t
                 s[u][i] = exp2_hw(__builtin_fmaf(s[u][i], c, -mu));
                 ls += s[u][i];
             }
-        l = __builtin_fmaf(l, al, ls);
-#pragma unroll
-        for (int i = 0; i < ND; i++)
-#pragma unroll
-            for (int e = 0; e < 16; e++) o[i][e] *= al;
+        l += ls;
 #pragma unroll
         for (int u = 0; u < NS; u++)
 #pragma unroll
-            for (int f = 0; f < 32 / KF; f++) {
+            for (int f = 0; f < FS; f++) {
                 const Frag pf = M::pack(s[u], f);
 #pragma unroll
-                for (int i = 0; i < ND; i++)
-                    o[i] = M::mma(M::load_tr(vs + 32 * u * LD + 32 * i, LD, f, lane), pf, o[i]);
+                for (int i = 0; i < ND; i++) o[i] = M::mma(TL::cols(vs, kg * BN + 32 * u, f, i, lane), pf, o[i]);
             }
+    };
+    auto step = [&](int i, const char* ks, const char* vs, char* kn, char* vn) ATTN_INLINE {
+        tiles_landed();
+        if (i + 1 < cnt) issue(tile_of(i + 1), kn, vn);
+        work(i, ks, vs);
+        if (i + 1 < cnt) commit(tile_of(i + 1), kn, vn);
+    };
+    commit(tile_of(0), ka, va);
+    for (int i = 0; i < cnt; i += 2) {
+        step(i, ka, va, kb, vb);
+        if (i + 1 < cnt) step(i + 1, kb, vb, ka, va);
     }
     l = half_sum(l);
     if constexpr (KG > 1) {
-        // the key groups' rows into group 0's, 32 columns of d at a time
-        float* jo = (float*)lds;
         if (half == 0) {
             sm[wave][lane] = m;
             sl[wave][lane] = l;
@@ -195,26 +222,9 @@ __global__ __launch_bounds__(kTreeThreads, DP * sizeof(T) <= 256 ? 2 : 1) void t
         const float mu = mt == -__builtin_inff() ? 0.0f : mt;
         l = 0.0f;
 #pragma unroll
-        for (int k = 0; k < KG; k++) l = __builtin_fmaf(sl[k * WR + wr][lane & 31], exp2_hw(sm[k * WR + wr][lane & 31] - mu), l);
-        const float f = exp2_hw(m - mu);
-#pragma unroll
-        for (int i = 0; i < ND; i++) {
-            __syncthreads();
-            if (kg) {
-#pragma unroll
-                for (int e = 0; e < 16; e++) jo[(((kg - 1) * WR + wr) * 16 + e) * 64 + lane] = o[i][e] * f;
-            }
-            __syncthreads();
-            if (!kg) {
-#pragma unroll
-                for (int e = 0; e < 16; e++) {
-                    float t = o[i][e] * f;
-#pragma unroll
-                    for (int k = 1; k < KG; k++) t += jo[(((k - 1) * WR + wr) * 16 + e) * 64 + lane];
-                    o[i][e] = t;
-                }
-            }
-        }
+        for (int k = 0; k < KG; k++)
+            l = __builtin_fmaf(sl[k * WR + wr][lane & 31], exp2_hw(sm[k * WR + wr][lane & 31] - mu), l);
+        join_groups<KG, WR, ND>(o, exp2_hw(m - mu), ka, wr, kg, lane);
         m = mt;
         if (kg) return;
     }
@@ -224,18 +234,20 @@ __global__ __launch_bounds__(kTreeThreads, DP * sizeof(T) <= 256 ? 2 : 1) void t
     const bool store = there && !(again >> (lane & 31) & 1);
     const float inv = l == 0.0f ? 0.0f : 1.0f / l;
     const bool whole = per >= tiles;                      // no other split has keys
-    float* po = a.part + (((long)b * a.kv_heads + g) * a.splits + split) * rows * (a.d + 2);
+    const long part = ((long)bg * a.splits + split) * rows;
+    float* po = a.part + part * a.d;
     if (whole) {
         if (store) attn_store<T, ND>(out, o, inv, a.d, half, a.vec_out);
     } else {
         if (there && half == 0) {
-            po[(long)r * (a.d + 2) + a.d] = m;
-            po[(long)r * (a.d + 2) + a.d + 1] = l;
+            float* ps = a.part + tree_stats(a) + 2 * (part + r);
+            ps[0] = m;
+            ps[1] = l;
         }
-        if (store) attn_store<float, ND>(po + (long)r * (a.d + 2), o, 1.0f, a.d, half, false);
+        if (store) attn_store<float, ND>(po + (long)r * a.d, o, 1.0f, a.d, half, a.d % 4 == 0);
     }
     for (; again; again &= again - 1) {
-        const int rl = __ffsll((unsigned long long)again) - 1, rr = (rb * WR + wr) * 32 + rl;
+        const int rl = __ffsll((unsigned long long)again) - 1, rr = rw + rl;
         const int t = rr / rep, hh = g * rep + rr % rep;
         const float mr = __shfl(m, rl), ir = __shfl(inv, rl);
         const T* q = (const T*)a.q + (long)b * a.sq_b + (long)t * a.sq_t + (long)hh * a.sq_h;
@@ -248,56 +260,81 @@ __global__ __launch_bounds__(kTreeThreads, DP * sizeof(T) <= 256 ? 2 : 1) void t
         if (whole)
             attn_again<T, DP, true>((T*)a.out + (((long)b * a.tokens + t) * a.heads + hh) * a.d, ir, a.d, ja, jb, w, vrow);
         else
-            attn_again<T, DP, true>(po + (long)rr * (a.d + 2), 1.0f, a.d, ja, jb, w, vrow);
+            attn_again<T, DP, true>(po + (long)rr * a.d, 1.0f, a.d, ja, jb, w, vrow);
     }
 }
 
-// Splits joined: a wave per row.
+// Splits joined: a thread per 4 values of a row.
 template <typename T>
 __global__ __launch_bounds__(kTreeThreads) void tree_join_kernel(const TreeArgs a, int tile) {
-    const int lane = threadIdx.x & 63, rep = a.heads / a.kv_heads, rows = rep * a.tokens;
-    const int r = blockIdx.x * kAttnWaves + (threadIdx.x >> 6), b = blockIdx.y / a.kv_heads, g = blockIdx.y % a.kv_heads;
-    if (r >= rows) return;
+    const int rep = a.heads / a.kv_heads, rows = rep * a.tokens, d4 = (a.d + 3) / 4;
+    const long i = (long)blockIdx.x * kTreeThreads + threadIdx.x;
+    const int bg = blockIdx.y, b = bg / a.kv_heads, g = bg % a.kv_heads;
     const int len = a.len[b];
-    if (len < 0 || (long)len + a.tokens > a.cap) return;
+    if (i >= (long)rows * d4 || len < 0 || (long)len + a.tokens > a.cap) return;
     const int tiles = (len + a.tokens + tile - 1) / tile, per = tree_per(tiles, a.splits);
     if (per >= tiles) return;                              // one split: it stored the rows itself
-    const int live = (tiles + per - 1) / per;
-    const float* p = a.part + ((long)b * a.kv_heads + g) * a.splits * rows * (a.d + 2) + (long)r * (a.d + 2);
-    const long step = (long)rows * (a.d + 2);
+    const int live = (tiles + per - 1) / per, r = (int)(i / d4), c = (int)(i % d4) * 4;
+    const float* po = a.part + ((long)bg * a.splits * rows + r) * a.d + c;
+    const float* ps = a.part + tree_stats(a) + ((long)bg * a.splits * rows + r) * 2;
+    const long so = (long)rows * a.d, ss = 2L * rows;
     float m = -__builtin_inff();
-    for (int s = lane; s < live; s += 64) m = fmaxf(m, p[s * step + a.d]);
-#pragma unroll
-    for (int o = 32; o; o >>= 1) m = fmaxf(m, __shfl_xor(m, o));
+#pragma unroll 4
+    for (int s = 0; s < live; s++) m = fmaxf(m, ps[s * ss]);
     if (m == -__builtin_inff()) m = 0.0f;
     float l = 0.0f, acc[4] = {};
+    const bool vec = a.d % 4 == 0;
+#pragma unroll 4
     for (int s = 0; s < live; s++) {
-        const float f = exp2_hw(p[s * step + a.d] - m);
-        l = __builtin_fmaf(f, p[s * step + a.d + 1], l);
+        const float f = exp2_hw(ps[s * ss] - m);
+        l = __builtin_fmaf(f, ps[s * ss + 1], l);
+        f32x4 v = {0.0f, 0.0f, 0.0f, 0.0f};
+        if (vec) {
+            v = *reinterpret_cast<const f32x4*>(po + s * so);
+        } else {
 #pragma unroll
-        for (int i = 0; i < 4; i++)
-            if (lane + 64 * i < a.d) acc[i] = __builtin_fmaf(f, p[s * step + lane + 64 * i], acc[i]);
+            for (int e = 0; e < 4; e++)
+                if (c + e < a.d) v[e] = po[s * so + e];
+        }
+#pragma unroll
+        for (int e = 0; e < 4; e++) acc[e] = __builtin_fmaf(f, v[e], acc[e]);
     }
     const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-    T* out = (T*)a.out + (((long)b * a.tokens + r / rep) * a.heads + g * rep + r % rep) * a.d;
+    T* out = (T*)a.out + (((long)b * a.tokens + r / rep) * a.heads + g * rep + r % rep) * a.d + c;
+    union { T e[4]; u32x2 v2; u32x4 v4; } u;
 #pragma unroll
-    for (int i = 0; i < 4; i++)
-        if (lane + 64 * i < a.d) out[lane + 64 * i] = Mma<T>::from_f32(acc[i] * inv);
+    for (int e = 0; e < 4; e++) u.e[e] = Mma<T>::from_f32(acc[e] * inv);
+    if (a.vec_out) {
+        if constexpr (sizeof(T) == 2) *reinterpret_cast<u32x2*>(out) = u.v2;
+        else *reinterpret_cast<u32x4*>(out) = u.v4;
+    } else {
+#pragma unroll
+        for (int e = 0; e < 4; e++)
+            if (c + e < a.d) out[e] = u.e[e];
+    }
 }
 
-// Rows of a wave set: one wave's 32 while all fit there, else four waves' 128;
-// d past 128 in fp32 leaves LDS for one key group only.
+// Row sets: one while all rows fit there (two where four groups' tiles do not
+// fit LDS), else four.
 struct TreePlan {
     int wr, tile, splits;
 };
+constexpr int tree_few_sets(int es, int dp) { return dp * es <= 256 ? 1 : dp * es <= 512 ? 2 : 4; }
 static TreePlan tree_plan(const TreeArgs& a, int dtype) {
     const int rows = a.heads / a.kv_heads * a.tokens, es = dtype == 0 ? 4 : 2;
-    const int dp = a.d <= 32 ? 32 : a.d <= 64 ? 64 : a.d <= 128 ? 128 : 256;
+    const int dp = a.d <= 32 ? 32 : a.d <= 64 ? 64 : a.d <= 96 ? 96 : a.d <= 128 ? 128 : 256;
     TreePlan p;
-    p.wr = rows <= 32 && dp * es <= 512 ? 1 : 4;
-    p.tile = tree_tile(es, p.wr);
+    p.wr = tree_few_sets(es, dp);
+    if (rows > 32 * p.wr) p.wr = 4;
+    p.tile = tree_tile(es, dp, p.wr);
     const long groups = (long)a.batch * a.kv_heads * ((rows + 32 * p.wr - 1) / (32 * p.wr));
-    const long most = (a.cap + p.tile - 1) / p.tile;
+    // two workgroups to a CU, but two tiles to each at least: 24 drafts over 2019
+    // positions in fp32 (32/4 heads of 64) 22.4 us in 32 splits, 32.5 in 64 and
+    // 23.4 in 16; 16 bf16 caches of up to 8001 (32/8 heads of 128) 168 us in 2,
+    // 196 in one
+    // (one row set's tile is four groups' already: a token over 515 positions in
+    // fp32, 8 heads of 64, 13.1 us in splits of one tile, 15.2 of two)
+    const long least = p.wr == kAttnWaves ? 2L * p.tile : p.tile, most = (a.cap + least - 1) / least;
     long s = (2 * device_cus() + groups - 1) / groups;
     if (s > most) s = most;
     if (s > 64) s = 64;
@@ -308,26 +345,24 @@ static TreePlan tree_plan(const TreeArgs& a, int dtype) {
 template <typename T, int DP>
 static void tree_launch_dp(const TreeArgs& a, const TreePlan& p, hipStream_t s) {
     const int rows = a.heads / a.kv_heads * a.tokens;
-    const dim3 grid(p.splits, (rows + 32 * p.wr - 1) / (32 * p.wr), a.batch * a.kv_heads);
-    if constexpr (DP * sizeof(T) <= 512) {
-        if (p.wr == 1) {
-            hipLaunchKernelGGL((tree_kernel<T, DP, 1>), grid, dim3(kTreeThreads), 0, s, a);
-            return;
-        }
-    }
-    hipLaunchKernelGGL((tree_kernel<T, DP, 4>), grid, dim3(kTreeThreads), 0, s, a);
+    const long units = ((long)p.splits * a.batch * a.kv_heads + 7) / 8 * 8;
+    const dim3 grid((unsigned)(units * ((rows + 32 * p.wr - 1) / (32 * p.wr))));
+    constexpr int FEW = tree_few_sets(sizeof(T), DP);
+    if (p.wr == FEW) hipLaunchKernelGGL((tree_kernel<T, DP, FEW>), grid, dim3(kTreeThreads), 0, s, a);
+    else hipLaunchKernelGGL((tree_kernel<T, DP, 4>), grid, dim3(kTreeThreads), 0, s, a);
 }
 
 template <typename T>
 static void tree_launch_t(const TreeArgs& a, const TreePlan& p, hipStream_t s) {
     if (a.d <= 32) tree_launch_dp<T, 32>(a, p, s);
     else if (a.d <= 64) tree_launch_dp<T, 64>(a, p, s);
+    else if (a.d <= 96) tree_launch_dp<T, 96>(a, p, s);
     else if (a.d <= 128) tree_launch_dp<T, 128>(a, p, s);
     else tree_launch_dp<T, 256>(a, p, s);
     if (p.splits > 1) {
-        const int rows = a.heads / a.kv_heads * a.tokens;
-        hipLaunchKernelGGL((tree_join_kernel<T>), dim3((rows + kAttnWaves - 1) / kAttnWaves, a.batch * a.kv_heads),
-                           dim3(kTreeThreads), 0, s, a, p.tile);
+        const long threads = (long)(a.heads / a.kv_heads) * a.tokens * ((a.d + 3) / 4);
+        hipLaunchKernelGGL((tree_join_kernel<T>), dim3((unsigned)((threads + kTreeThreads - 1) / kTreeThreads),
+                           a.batch * a.kv_heads), dim3(kTreeThreads), 0, s, a, p.tile);
     }
 }
 

@@ -20,6 +20,7 @@ is no CPU path.
 from __future__ import annotations
 
 import ctypes
+import functools
 import os
 from typing import List, Optional, Tuple
 
@@ -1109,8 +1110,17 @@ def _fresh_or(out: Optional[torch.Tensor], shape, ref: torch.Tensor) -> torch.Te
 
 def _call(name: str, ref: torch.Tensor, *args) -> None:
     """The entry point on ref's device and torch's current stream there."""
-    with torch.cuda.device(ref.device):
-        check(getattr(_lib.load(), name)(*args, _stream(ref)), name)
+    if ref.device.index != torch.cuda.current_device():
+        with torch.cuda.device(ref.device):
+            return _call(name, ref, *args)
+    rc = getattr(_lib.load(), name)(*args, _stream(ref))
+    if rc:
+        check(rc, name)
+
+
+@functools.lru_cache(maxsize=None)
+def _default_scale(head_dim: int) -> float:
+    return attention_scale(head_dim)
 
 
 def _packed_checks(q, k, v, cu_seqlens):
@@ -1154,7 +1164,7 @@ def packed_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqle
     fresh = out is None
     out = _fresh_or(out, q.shape, q)
     lse = torch.empty((H, total), device=q.device, dtype=torch.float32) if return_lse else None
-    scale = attention_scale(D) if scale is None else float(scale)
+    scale = _default_scale(D) if scale is None else float(scale)
     if total:
         _call("rac_packed_attention_dev", q, q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(),
               lse.data_ptr() if lse is not None else None, cu.data_ptr(), cu.numel() - 1, total, H, k.size(1), D,
@@ -1180,7 +1190,7 @@ def packed_attention_backward(grad_out: torch.Tensor, q: torch.Tensor, k: torch.
     grad_out, out = grad_out.contiguous(), out.contiguous()
     dq = torch.empty(q.shape, device=q.device, dtype=q.dtype)
     dk, dv = (torch.empty(k.shape, device=q.device, dtype=q.dtype) for _ in range(2))
-    scale = attention_scale(D) if scale is None else float(scale)
+    scale = _default_scale(D) if scale is None else float(scale)
     if total:
         ws = torch.empty(_lib.load().rac_packed_attention_backward_workspace_bytes(total, H) // 4, device=q.device,
                          dtype=torch.float32)
@@ -1232,7 +1242,7 @@ def tree_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor
         raise RuntimeError("RAC: parents must be [T] or [batch, T]")
     q, k, v = _unit_last(q), _unit_last(k_cache), _unit_last(v_cache)
     res = _fresh_or(out, (T, H, D) if single else (B, T, H, D), q)
-    scale = attention_scale(D) if scale is None else float(scale)
+    scale = _default_scale(D) if scale is None else float(scale)
     if B:
         n = _lib.load().rac_tree_attention_workspace_bytes(B, T, H, G, D, cap, dt)
         ws = torch.empty(n // 4, device=q.device, dtype=torch.float32) if n else None

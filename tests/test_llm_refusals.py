@@ -109,7 +109,7 @@ def test_nothing_to_do_is_no_error(lib):
 
 
 def test_workspace_sizes(lib):
-    assert lib.rac_packed_attention_backward_workspace_bytes(100, 8) == 3200
+    assert lib.rac_packed_attention_backward_workspace_bytes(100, 8) == 6400
     assert lib.rac_packed_attention_backward_workspace_bytes(0, 8) == 0
     assert lib.rac_tree_attention_workspace_bytes(0, 4, 4, 2, 64, 100, 0) == 0
     assert lib.rac_tree_attention_workspace_bytes(1, 300, 4, 2, 64, 1000, 0) == 0
