@@ -212,6 +212,8 @@ class RACError(RuntimeError):
 def load(path: str | None = None) -> ctypes.CDLL:
     """Load librac_amd.so (once) and declare every exported signature."""
     global _lib
+    if path is None and _lib is not None:
+        return _lib
     with _lock:
         if _lib is not None and path is None:
             return _lib

@@ -15,8 +15,7 @@
 //
 // The list lives one entry to a lane, best first: keys are the logits' bits
 // mapped to integers in their order (NaN as -inf, -0 as 0), equal keys go to
-// the lower token.  Lanes offer their values in token order, so that a later
-// value enters only if it is larger than the last entry.
+// the lower token.
 #include <hip/hip_runtime.h>
 #include "rac_internal.hpp"
 #include "rac_mma.hpp"
@@ -30,12 +29,7 @@ __device__ __forceinline__ uint32_t lp_key(float x) {
     const uint32_t u = __builtin_bit_cast(uint32_t, x + 0.0f);
     return (int32_t)u < 0 ? ~u : u | 0x80000000u;
 }
-// the same of bits that are uniform, on the scalar side
-__device__ __forceinline__ uint32_t lp_key_bits(uint32_t u) {
-    if ((u & 0x7fffffffu) > 0x7f800000u) u = 0xff800000u;
-    if (u == 0x80000000u) u = 0;
-    return (int32_t)u < 0 ? ~u : u | 0x80000000u;
-}
+constexpr uint32_t kLpLowest = 0x007fffffu;              // -inf's key
 __device__ __forceinline__ float lp_value(uint32_t k) {
     return __builtin_bit_cast(float, (int32_t)k < 0 ? k & 0x7fffffffu : ~k);
 }
@@ -57,6 +51,13 @@ __device__ __forceinline__ void lp_join(LpStat& a, float m, float l, float s) {
     a.m = mt;
 }
 
+// the wave's own LDS writes are there for its other lanes' reads
+__device__ __forceinline__ void wave_lds_sync() {
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront", "local");
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront", "local");
+}
+
 // the wave's lanes joined, the same bits in all
 __device__ __forceinline__ void lp_wave_join(LpStat& r) {
     const int lane = threadIdx.x & 63;
@@ -70,68 +71,97 @@ __device__ __forceinline__ void lp_wave_join(LpStat& r) {
     }
 }
 
-// the value of the lane below (lane 0 keeps its own)
-__device__ __forceinline__ int lane_below(int v) {
-    return __builtin_amdgcn_update_dpp(v, v, 0x138, 0xf, 0xf, false);        // wave_shr:1
+// An entry of a list: the key above, and the token so that of equal keys the
+// lower one is the larger entry; 0 is none.
+typedef unsigned long long lp_t;
+__device__ __forceinline__ lp_t lp_entry(uint32_t key, int tok) {
+    return (lp_t)key << 32 | (uint32_t)(0x7fffffff - tok);
+}
+__device__ __forceinline__ float lp_entry_value(lp_t e) { return lp_value((uint32_t)(e >> 32)); }
+__device__ __forceinline__ int lp_entry_token(lp_t e) { return 0x7fffffff - (int)(uint32_t)e; }
+__device__ __forceinline__ lp_t lp_lane(lp_t v, int lane) {                      // lane uniform
+    return (lp_t)(uint32_t)__builtin_amdgcn_readlane((int)(v >> 32), lane) << 32 |
+           (uint32_t)__builtin_amdgcn_readlane((int)v, lane);
 }
 
-// entry (key, tok) into the wave's list
-__device__ __forceinline__ void lp_insert(uint32_t& lk, int& lt, uint32_t key, int tok, int lane) {
-    const int at = __popcll(__ballot(lk > key || (lk == key && lt < tok)));
-    const uint32_t pk = (uint32_t)lane_below((int)lk);
-    const int pt = lane_below(lt);
-    lk = lane == at ? key : lane > at ? pk : lk;
-    lt = lane == at ? tok : lane > at ? pt : lt;
+// entry e (uniform) into the wave's list, best first, one to a lane
+__device__ __forceinline__ void lp_insert(lp_t& list, lp_t e, int lane) {
+    const int at = __popcll(__ballot(list > e));
+    // the entry of the lane below (wave_shr:1)
+    const int hi = (int)(list >> 32), lo = (int)list;
+    const lp_t below = (lp_t)(uint32_t)__builtin_amdgcn_update_dpp(hi, hi, 0x138, 0xf, 0xf, false) << 32 |
+                       (uint32_t)__builtin_amdgcn_update_dpp(lo, lo, 0x138, 0xf, 0xf, false);
+    list = lane == at ? e : lane > at ? below : list;
 }
 
-// A threshold that at least `top` of the wave's values exceed (0: none such):
-// just below the top-th largest of the lanes' own maxima.
+// how many of the n entries at p (LDS, best first) beat e
+__device__ __forceinline__ int lp_above(const lp_t* p, int n, lp_t e) {
+    int lo = 0;
+    for (int step = 32; step; step >>= 1)
+        if (lo + step <= n && p[lo + step - 1] > e) lo += step;
+    return lo == 63 && n == 64 && p[63] > e ? 64 : lo;
+}
+
+// The wave's c entries of no order, one to each of its first lanes, best first:
+// each counts those that beat it, with no step waiting for the one before.
+// buf: 64 entries of LDS of the wave's own.
+__device__ __forceinline__ lp_t lp_sort(lp_t e, int c, lp_t* buf, int lane) {
+    int rank = 0;
+#pragma unroll 4
+    for (int i = 0; i < c; i++) rank += lp_lane(e, i) > e;
+    wave_lds_sync();
+    if (lane < c) buf[rank] = e;
+    wave_lds_sync();
+    return lane < c ? buf[lane] : 0;
+}
+
+// the best `top` of two lists (c entries in `more`), each best first
+__device__ __forceinline__ void lp_merge(lp_t& list, lp_t more, int top, int c, lp_t* buf, lp_t* buf2, int lane) {
+    wave_lds_sync();
+    buf[lane] = list;
+    buf2[lane] = more;
+    wave_lds_sync();
+    const int a = lane + lp_above(buf2, c, list), b = lane + lp_above(buf, top, more);
+    wave_lds_sync();
+    if (lane < top && a < top) buf[a] = list;
+    if (lane < c && b < top) buf[b] = more;
+    wave_lds_sync();
+    list = lane < top ? buf[lane] : 0;
+}
+
+// A key that at least `top` of the wave's values reach: the top-th largest of
+// the lanes' own maxima, in its upper 16 bits.
 __device__ __forceinline__ uint32_t lp_start(uint32_t mine, int top) {
-    int above = 0;
-    for (int i = 0; i < 64; i++) {
-        const uint32_t k = (uint32_t)__builtin_amdgcn_readlane((int)mine, i);
-        above += k > mine || (k == mine && i < (int)(threadIdx.x & 63));
+    uint32_t t = 0;
+#pragma unroll
+    for (int bit = 31; bit >= 16; bit--) {
+        const uint32_t more = t | 1u << bit;
+        if (__popcll(__ballot(mine >= more)) >= top) t = more;
     }
-    const uint64_t at = __ballot(above == top - 1);
-    const uint32_t k = (uint32_t)__builtin_amdgcn_readlane((int)mine, __ffsll((unsigned long long)at) - 1);
-    return k ? k - 1 : 0;
+    return t;
 }
 
-// the lists of the workgroup's waves into the `top` best, rank by rank
-__device__ __forceinline__ void lp_rank(uint32_t lk, int lt, int top, uint32_t (*sk)[kLogprobMaxTop],
-                                        int (*st)[kLogprobMaxTop], uint32_t* ok, int* ot) {
+// the lists of the workgroup's waves into the `top` best, out[rank]
+__device__ __forceinline__ void lp_rank(lp_t list, int top, lp_t (*all)[kLogprobMaxTop], lp_t* out) {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    sk[wave][lane] = lk;
-    st[wave][lane] = lt;
+    all[wave][lane] = list;
     __syncthreads();
-    if (lane < top) {
-        int rank = 0;
+    int rank = lane;
 #pragma unroll
-        for (int w = 0; w < kLpWaves; w++)
-            for (int i = 0; i < top; i += 4) {
-                const u32x4 k4 = *reinterpret_cast<const u32x4*>(&sk[w][i]);
-                const u32x4 t4 = *reinterpret_cast<const u32x4*>(&st[w][i]);
-#pragma unroll
-                for (int j = 0; j < 4; j++) {
-                    // empty entries alike but for their place
-                    const uint32_t k = k4[j];
-                    const int t = (int)t4[j];
-                    rank += i + j < top &&
-                            (k > lk || (k == lk && (t < lt || (t == lt && 64 * w + i + j < 64 * wave + lane))));
-                }
-            }
-        if (rank < top) {
-            ok[rank] = lk;
-            ot[rank] = lt;
-        }
+    for (int w = 1; w < kLpWaves; w++) {
+        const int o = (wave + w) % kLpWaves;
+        // empty entries behind those of the waves before
+        int n = lp_above(all[o], top, list);
+        if (list == 0 && o < wave) n = top;
+        rank += n;
     }
+    if (lane < top && rank < top) out[rank] = list;
     __syncthreads();
 }
 
 // row results from the whole row's statistics
 template <typename T>
-__device__ __forceinline__ void lp_finish(const LogprobArgs& a, long row, const LpStat& r, const uint32_t* ok,
-                                          const int* ot) {
+__device__ __forceinline__ void lp_finish(const LogprobArgs& a, long row, const LpStat& r, const lp_t* best) {
     const bool empty = r.m == -__builtin_inff() && r.l == 0.0f;
     const float ll = __builtin_logf(r.l), lse = empty ? -__builtin_inff() : __builtin_fmaf(r.m, kLpLn2, ll);
     auto logp = [&](float x) {
@@ -147,19 +177,21 @@ __device__ __forceinline__ void lp_finish(const LogprobArgs& a, long row, const 
         if (a.lse) a.lse[row] = lse;
     }
     if ((int)threadIdx.x < a.top) {
-        a.top_lp[row * a.top + threadIdx.x] = logp(lp_value(ok[threadIdx.x]));
-        a.top_tok[row * a.top + threadIdx.x] = ot[threadIdx.x];
+        a.top_lp[row * a.top + threadIdx.x] = logp(lp_entry_value(best[threadIdx.x]));
+        a.top_tok[row * a.top + threadIdx.x] = lp_entry_token(best[threadIdx.x]);
     }
 }
+
+// floats of a split's part: three statistics, a gap, `top` entries
+__host__ __device__ constexpr int lp_width(int top) { return 4 + 2 * top; }
 
 // One workgroup per row and split: columns [c0, c1) of the row.
 template <typename T, bool TOP>
 __global__ __launch_bounds__(kLpThreads) void logprob_kernel(const LogprobArgs a) {
     constexpr int VEC = Mma<T>::VEC, U = 4;                // U vectors of a thread in flight
-    __shared__ __attribute__((aligned(16))) uint32_t sk[TOP ? kLpWaves : 1][kLogprobMaxTop], ok[kLogprobMaxTop];
-    __shared__ __attribute__((aligned(16))) int st[TOP ? kLpWaves : 1][kLogprobMaxTop], ot[kLogprobMaxTop];
+    __shared__ lp_t all[TOP ? kLpWaves : 1][kLogprobMaxTop], two[TOP ? kLpWaves : 1][64], best[kLogprobMaxTop];
     __shared__ float red[kLpWaves][3];
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const long row = blockIdx.x;
     const int split = blockIdx.y;
     const T* x = (const T*)a.x + row * a.stride;
@@ -168,9 +200,8 @@ __global__ __launch_bounds__(kLpThreads) void logprob_kernel(const LogprobArgs a
     const long nv = (a.vocab + off + VEC - 1) / VEC, per = (nv + a.splits - 1) / a.splits;
     const long v0 = split * per, v1 = v0 + per < nv ? v0 + per : nv;
     LpStat r = {-__builtin_inff(), 0.0f, 0.0f};
-    uint32_t lk = 0;                                       // 0: nothing yet
-    int lt = 0x7fffffff;
-    uint32_t thr = 0;
+    lp_t list = 0, last = 0;                               // its last entry: what a value has to beat
+    uint32_t thr = 0;                                      // the key that it has to reach
     for (long b = v0; b < v1; b += U * kLpThreads) {
         float f[U][VEC];
 #pragma unroll
@@ -195,36 +226,50 @@ __global__ __launch_bounds__(kLpThreads) void logprob_kernel(const LogprobArgs a
                 mx = fmaxf(mx, f[u][e]);
             }
         if constexpr (TOP) {
-            if (__any(lp_key(mx) > thr)) {
-                // keys of places past the row are never offered, but count as
-                // -inf here, which at worst is too low a threshold
-                if (b == v0) thr = lp_start(lp_key(mx), a.top);
+            const uint32_t mk = lp_key(mx);
+            if (b == v0) thr = lp_start(mk, a.top);
+            // NaN beside a number counts as -inf, which a maximum hides
+            if (__any(mk >= thr) || thr <= kLpLowest) {
+                lp_t* const cand = all[wave];
+                int c = 0;
 #pragma unroll
                 for (int u = 0; u < U; u++) {
                     float um = f[u][0];
 #pragma unroll
                     for (int e = 1; e < VEC; e++) um = fmaxf(um, f[u][e]);
-                    const long v = b + u * kLpThreads + tid, c = v * VEC - off;
-                    const uint32_t uk = v < v1 ? lp_key(um) : 0;
-                    for (uint64_t cand = __ballot(uk > thr); cand;) {
-                        const int src = __ffsll((unsigned long long)cand) - 1;
+                    const long v = b + u * kLpThreads + tid;
+                    const int t0 = (int)(v * VEC - off);
+                    if (!__any(v < v1 && lp_key(um) >= thr) && thr > kLpLowest) continue;
 #pragma unroll
-                        for (int e = 0; e < VEC; e++) {
-                            const float fe = f[u][e];
-                            const uint32_t key = lp_key_bits(__builtin_amdgcn_readlane(__builtin_bit_cast(int, fe), src));
-                            if (key > thr) {
-                                const int tok = __builtin_amdgcn_readlane((int)(c + e), src);
-                                if (tok >= 0 && tok < a.vocab) {
-                                    lp_insert(lk, lt, key, tok, lane);
-                                    const uint32_t last = __builtin_amdgcn_readlane(lk, a.top - 1);
-                                    if (last > thr) thr = last;
-                                }
-                            }
+                    for (int e = 0; e < VEC; e++) {
+                        const uint32_t key = lp_key(f[u][e]);
+                        const int tok = t0 + e;
+                        const lp_t entry = lp_entry(key, tok);
+                        const bool in = v < v1 && tok >= 0 && tok < a.vocab && key >= thr && entry > last;
+                        const uint64_t at = __ballot(in);
+                        if (!at) continue;
+                        const int place = c + __popcll(at & ((1ull << lane) - 1));
+                        if (in && place < 64) cand[place] = entry;
+                        c += __popcll(at);
+                        if (c > 64) {
+                            // what has no place goes into the list by itself
+                            for (uint64_t rest = __ballot(in && place >= 64); rest; rest &= rest - 1)
+                                lp_insert(list, lp_lane(entry, __ffsll((unsigned long long)rest) - 1), lane);
+                            c = 64;
                         }
-                        // the lanes behind that still have one
-                        cand = src == 63 ? 0 : __ballot(uk > thr) & (~0ull << (src + 1));
                     }
                 }
+                wave_lds_sync();
+                lp_t more = lane < c ? cand[lane] : 0;
+                if (c > 2) {
+                    more = lp_sort(more, c, cand, lane);
+                    lp_merge(list, more, a.top, c, cand, two[wave], lane);
+                } else {
+                    for (int i = 0; i < c; i++) lp_insert(list, lp_lane(more, i), lane);
+                }
+                last = lp_lane(list, a.top - 1);
+                // a later batch's equal key has a higher token
+                if ((uint32_t)(last >> 32) >= thr) thr = (uint32_t)(last >> 32) + 1;
             }
         }
         mx *= kLog2e;
@@ -255,67 +300,61 @@ __global__ __launch_bounds__(kLpThreads) void logprob_kernel(const LogprobArgs a
         red[wave][1] = r.l;
         red[wave][2] = r.s;
     }
-    if constexpr (TOP) lp_rank(lk, lt, a.top, sk, st, ok, ot);
+    if constexpr (TOP) lp_rank(lane < a.top ? list : 0, a.top, all, best);
     else __syncthreads();
     r = {red[0][0], red[0][1], red[0][2]};
 #pragma unroll
     for (int w = 1; w < kLpWaves; w++) lp_join(r, red[w][0], red[w][1], red[w][2]);
     if (a.splits == 1) {
-        lp_finish<T>(a, row, r, ok, ot);
+        lp_finish<T>(a, row, r, best);
         return;
     }
-    float* p = a.part + (row * a.splits + split) * (3 + 2 * a.top);
+    float* p = a.part + (row * a.splits + split) * lp_width(a.top);
     if (tid == 0) {
         p[0] = r.m;
         p[1] = r.l;
         p[2] = r.s;
     }
-    if (TOP && tid < a.top) {
-        reinterpret_cast<uint32_t*>(p)[3 + tid] = ok[tid];
-        reinterpret_cast<int*>(p)[3 + a.top + tid] = ot[tid];
-    }
+    if (TOP && tid < a.top) reinterpret_cast<lp_t*>(p + 4)[tid] = best[tid];
 }
 
 // The splits of a row joined.
 template <typename T, bool TOP>
 __global__ __launch_bounds__(kLpThreads) void logprob_join_kernel(const LogprobArgs a) {
-    __shared__ __attribute__((aligned(16))) uint32_t sk[TOP ? kLpWaves : 1][kLogprobMaxTop], ok[kLogprobMaxTop];
-    __shared__ __attribute__((aligned(16))) int st[TOP ? kLpWaves : 1][kLogprobMaxTop], ot[kLogprobMaxTop];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    __shared__ lp_t all[TOP ? kLpWaves : 1][kLogprobMaxTop], two[TOP ? kLpWaves : 1][64], best[kLogprobMaxTop];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const long row = blockIdx.x;
-    const int width = 3 + 2 * a.top;
+    const int width = lp_width(a.top);
     const float* p = a.part + row * a.splits * width;
+    lp_t list = 0, more = 0;
+    // the wave's first list as it stands; the next one's load ahead of its turn
+    auto load = [&](int s) {
+        return s < a.splits && lane < a.top ? reinterpret_cast<const lp_t*>(p + (long)s * width + 4)[lane] : 0;
+    };
+    if constexpr (TOP) {
+        list = load(wave);
+        more = load(wave + kLpWaves);
+    }
     LpStat r = {-__builtin_inff(), 0.0f, 0.0f};
-    for (int s = lane; s < a.splits; s += 64) lp_join(r, p[s * width], p[s * width + 1], p[s * width + 2]);
+    for (int s = lane; s < a.splits; s += 64) {
+        const float* q = p + (long)s * width;
+        lp_join(r, q[0], q[1], q[2]);
+    }
     lp_wave_join(r);
     if constexpr (TOP) {
-        // the wave's first list as it stands; the next one's loads ahead of its turn
-        const uint32_t* list = reinterpret_cast<const uint32_t*>(p) + 3;
-        auto load = [&](int s, uint32_t& k, int& t) {
-            const bool there = s < a.splits && lane < a.top;
-            k = there ? list[s * width + lane] : 0;
-            t = there ? (int)list[s * width + a.top + lane] : 0x7fffffff;
-        };
-        uint32_t lk, mk;
-        int lt, mt;
-        load(wave, lk, lt);
-        load(wave + kLpWaves, mk, mt);
         for (int s = wave + kLpWaves; s < a.splits; s += kLpWaves) {
-            uint32_t nk;
-            int nt;
-            load(s + kLpWaves, nk, nt);
-            for (int i = 0; i < a.top; i++) {
-                const uint32_t key = __builtin_amdgcn_readlane(mk, i);
-                // splits come in token order: an equal key's token is higher
-                if (key <= __builtin_amdgcn_readlane(lk, a.top - 1)) break;
-                lp_insert(lk, lt, key, __builtin_amdgcn_readlane(mt, i), lane);
+            const lp_t next = load(s + kLpWaves);
+            const int c = __popcll(__ballot(more > lp_lane(list, a.top - 1)));
+            if (c > 2) {
+                lp_merge(list, more, a.top, c, all[wave], two[wave], lane);
+            } else {
+                for (int i = 0; i < c; i++) lp_insert(list, lp_lane(more, i), lane);
             }
-            mk = nk;
-            mt = nt;
+            more = next;
         }
-        lp_rank(lk, lt, a.top, sk, st, ok, ot);
+        lp_rank(lane < a.top ? list : 0, a.top, all, best);
     }
-    lp_finish<T>(a, row, r, ok, ot);
+    lp_finish<T>(a, row, r, best);
 }
 
 // dx of a piece of a row: VEC values a thread and step.
@@ -379,7 +418,7 @@ static int logprob_splits(long rows, long vocab) {
 
 long token_logprobs_workspace(long rows, long vocab, int top, int dtype) {
     const int s = logprob_splits(rows, vocab);
-    return s > 1 ? 4L * rows * s * (3 + 2 * top) : 0;
+    return s > 1 ? 4L * rows * s * lp_width(top) : 0;
 }
 
 template <typename T>

@@ -1110,10 +1110,11 @@ def _fresh_or(out: Optional[torch.Tensor], shape, ref: torch.Tensor) -> torch.Te
 
 def _call(name: str, ref: torch.Tensor, *args) -> None:
     """The entry point on ref's device and torch's current stream there."""
-    if ref.device.index != torch.cuda.current_device():
-        with torch.cuda.device(ref.device):
+    index = ref.device.index
+    if index != torch.cuda.current_device():
+        with torch.cuda.device(index):
             return _call(name, ref, *args)
-    rc = getattr(_lib.load(), name)(*args, _stream(ref))
+    rc = getattr(_lib.load(), name)(*args, torch._C._cuda_getCurrentRawStream(index))
     if rc:
         check(rc, name)
 
@@ -1129,12 +1130,13 @@ def _packed_checks(q, k, v, cu_seqlens):
         _like(t, q, n)
         if t.dtype != q.dtype:
             raise RuntimeError("RAC: q, k and v must have the same dtype")
-    if q.dim() != 3 or k.dim() != 3 or k.shape != v.shape or q.size(0) != k.size(0) or q.size(2) != k.size(2):
+    qs, ks = q.shape, k.shape
+    if len(qs) != 3 or len(ks) != 3 or ks != v.shape or qs[0] != ks[0] or qs[2] != ks[2]:
         raise RuntimeError("RAC: packed_attention expects q [total, n_heads, d_head], k and v "
                            "[total, n_kv_heads, d_head]")
-    if k.size(1) == 0 or q.size(1) == 0 or q.size(1) % k.size(1):
+    if ks[1] == 0 or qs[1] == 0 or qs[1] % ks[1]:
         raise RuntimeError("RAC: n_heads must be a multiple of n_kv_heads")
-    if not 0 < q.size(2) <= LLM_MAX_HEAD:
+    if not 0 < qs[2] <= LLM_MAX_HEAD:
         raise RuntimeError(f"RAC: d_head must be in [1, {LLM_MAX_HEAD}]")
     cu = _require_int32(cu_seqlens, q, "cu_seqlens")
     if cu.dim() != 1 or cu.numel() < 1:
