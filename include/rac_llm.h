@@ -50,8 +50,9 @@ int rac_packed_attention_dev(const void *q, const void *k, const void *v, void *
  * n_kv_heads, d_head] contiguous, lse as the forward pass left it.  dk and dv
  * are sums over the query heads that share a head, taken in a fixed order: the
  * same call gives the same bits.  workspace:
- * rac_packed_attention_backward_workspace_bytes bytes. */
-long rac_packed_attention_backward_workspace_bytes(int total, int n_heads);
+ * rac_packed_attention_backward_workspace_bytes bytes on a 16-byte boundary, the
+ * call's own while it runs. */
+long rac_packed_attention_backward_workspace_bytes(int n_seqs, int total, int n_heads, int n_kv_heads, int d_head);
 int rac_packed_attention_backward_dev(const void *q, const void *k, const void *v, const void *out,
                                       const void *grad_out, const float *lse, const int *cu_seqlens, void *dq,
                                       void *dk, void *dv, float *workspace, int n_seqs, int total, int n_heads,

@@ -512,7 +512,7 @@ RAC_EXPORT int rac_packed_attention_dev(const void* q, const void* k, const void
                                         int zero_rest, int dtype, void* stream) {
     const char* who = "rac_packed_attention_dev";
     if (!q || !k || !v || !out || !cu_seqlens) return fail(RAC_ERR_NULL_PTR, "%s: null buffer", who);
-    PackedArgs a{q, k, v, nullptr, out, nullptr, nullptr, nullptr, lse, nullptr, cu_seqlens, n_seqs, total, n_heads,
+    PackedArgs a{q, k, v, nullptr, out, nullptr, nullptr, nullptr, lse, nullptr, nullptr, cu_seqlens, n_seqs, total, n_heads,
                  n_kv_heads, d_head, q_stride, q_head_stride, k_stride, k_head_stride, v_stride, v_head_stride, scale,
                  zero_rest, false, false};
     const int rc = packed_args(who, &a, dtype);
@@ -523,8 +523,18 @@ RAC_EXPORT int rac_packed_attention_dev(const void* q, const void* k, const void
     return check_hip(packed_fwd_launch(a, dtype, (hipStream_t)stream), "rac_packed_attention_dev launch");
 }
 
-RAC_EXPORT long rac_packed_attention_backward_workspace_bytes(int total, int n_heads) {
-    return total > 0 && n_heads > 0 ? 8L * total * n_heads : 0;
+RAC_EXPORT long rac_packed_attention_backward_workspace_bytes(int n_seqs, int total, int n_heads, int n_kv_heads,
+                                                              int d_head) {
+    PackedArgs a{};
+    a.n_seqs = n_seqs;
+    a.total = total;
+    a.heads = n_heads;
+    a.kv_heads = n_kv_heads;
+    a.d = d_head;
+    a.scale = 1.0f;
+    if (packed_args("rac_packed_attention_backward_workspace_bytes", &a, 0) || total == 0) return 0;
+    // the parts behind the rows' statistics, on a 16-byte boundary
+    return 4L * ((2L * total * n_heads + 3) / 4 * 4 + packed_dkv_parts(a));
 }
 
 RAC_EXPORT int rac_packed_attention_backward_dev(const void* q, const void* k, const void* v, const void* out,
@@ -537,7 +547,8 @@ RAC_EXPORT int rac_packed_attention_backward_dev(const void* q, const void* k, c
     const char* who = "rac_packed_attention_backward_dev";
     if (!q || !k || !v || !out || !grad_out || !lse || !cu_seqlens || !dq || !dk || !dv || !workspace)
         return fail(RAC_ERR_NULL_PTR, "%s: null buffer", who);
-    PackedArgs a{q, k, v, grad_out, const_cast<void*>(out), dq, dk, dv, const_cast<float*>(lse), workspace, cu_seqlens,
+    PackedArgs a{q, k, v, grad_out, const_cast<void*>(out), dq, dk, dv, const_cast<float*>(lse), workspace,
+                 workspace + (2L * total * n_heads + 3) / 4 * 4, cu_seqlens,
                  n_seqs, total, n_heads, n_kv_heads, d_head, q_stride, q_head_stride, k_stride, k_head_stride, v_stride,
                  v_head_stride, scale, zero_rest, false, false};
     const int rc = packed_args(who, &a, dtype);

@@ -187,7 +187,8 @@ hipError_t swiglu_launch(const float* gu, float* out, long n, int iters, hipStre
 // k and v [total, kv_heads, d] with element strides per row (_t) and head (_h);
 // out, grad, dq [total, heads, d], dk, dv [total, kv_heads, d] contiguous; lse
 // [heads, total]; stats [heads, total, 2]: log2 of the sums (of rows without any:
-// +inf) and D = do . o.  vec: every row of q, k, v (and out, grad in a backward
+// +inf) and D = do . o; part: dk and dv of every query head in fp32, each [total,
+// heads, d] (null: packed_dkv_parts is 0).  vec: every row of q, k, v (and out, grad in a backward
 // pass) is 16-byte aligned and d whole 16-byte vectors; vec_out: the outputs'
 // rows take stores of 4 values.  zero_rest: rows outside every sequence become 0.
 // dtype 0 fp32, 1 bf16, 2 fp16; d <= kPackedMaxHead.
@@ -195,7 +196,7 @@ constexpr int kPackedMaxHead = 256;
 struct PackedArgs {
     const void *q, *k, *v, *grad;
     void *out, *dq, *dk, *dv;
-    float *lse, *stats;
+    float *lse, *stats, *part;
     const int* cu;
     int n_seqs, total, heads, kv_heads, d;
     long sq_t, sq_h, sk_t, sk_h, sv_t, sv_h;
@@ -205,6 +206,7 @@ struct PackedArgs {
 };
 hipError_t packed_fwd_launch(const PackedArgs& a, int dtype, hipStream_t s);
 hipError_t packed_dq_launch(const PackedArgs& a, int dtype, hipStream_t s);     // and a.stats
+long packed_dkv_parts(const PackedArgs& a);          // floats of a.part
 hipError_t packed_dkv_launch(const PackedArgs& a, int dtype, hipStream_t s);    // reads a.stats
 // Attention of drafted tokens over a cache (rac_tree.hip): q [batch, tokens,
 // heads, d], caches [batch, kv_heads, cap, d], element strides; out contiguous

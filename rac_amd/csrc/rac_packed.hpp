@@ -139,10 +139,10 @@ __device__ __forceinline__ void packed_zero(T* p, int row0, int rows, int heads,
 // the workgroups, with a critical path as much shorter, and pay with LDS and a
 // sum over the groups at the end.
 // Rows of the other side a wave takes from a tile, and a tile's.
-template <typename T, int DP, int WR, int MOST = 64>
+template <typename T, int DP, int WR>
 struct PackedShape {
     static constexpr int KG = kAttnWaves / WR;
-    static constexpr int BN = sizeof(T) == 2 && WR == 4 && DP <= 128 ? (DP % 64 ? 64 : MOST) : 32;
+    static constexpr int BN = sizeof(T) == 2 && WR == 4 && DP <= 128 ? 64 : 32;
     static constexpr int TILE = BN * KG, BYTES = TILE * DP * (int)sizeof(T), ROWS = 32 * WR;
     static constexpr int ND = DP / 32, NF = DP / Mma<T>::KF, NS = BN / 32, FS = 32 / Mma<T>::KF;
 };
@@ -150,18 +150,41 @@ struct PackedShape {
 // tiles of `rows` rows: at most this many, whatever the sequences' lengths
 inline long packed_tiles(const PackedArgs& a, int rows) { return (long)a.total / rows + a.n_seqs + 2; }
 
-// Row sets of a workgroup: 4 while that makes a workgroup for every CU, else as
-// few as LDS allows (128 KB of it hold the two tiles twice).
+// LDS for the two tiles twice: 128 KB of it
 template <typename T, int DP, int WR>
 constexpr bool packed_fits() {
     return 4 * PackedShape<T, DP, WR>::BYTES <= (128 << 10);
 }
+// the fewest row sets (16-bit rows of 192 bytes and more: 128 KB to a workgroup
+// cost more than its shorter path gains, 3 prompts of 2500 rows, 8 heads of
+// 128, 39 us in one set, 22 in two)
 template <typename T, int DP>
 constexpr int packed_few_sets() {
+    if (sizeof(T) == 2 && DP >= 96) return 2;
     return packed_fits<T, DP, 1>() ? 1 : packed_fits<T, DP, 2>() ? 2 : 4;
 }
-inline bool packed_few(const PackedArgs& a, int heads) {
-    return ((long)a.total / 128 + (a.n_seqs + 1) / 2) * heads < device_cus();
+// about `each` workgroups for every CU, with `rows` rows to one
+inline bool packed_enough(const PackedArgs& a, int rows, int heads, int each) {
+    return ((long)a.total / rows + (a.n_seqs + 1) / 2) * heads >= each * device_cus();
+}
+// Whether the keys' kernel takes a workgroup for every query head, and a join:
+// where heads share keys and the keys' tiles alone leave CUs idle.
+inline bool packed_by_head_parts(const PackedArgs& a) {
+    return a.heads > a.kv_heads && !packed_enough(a, 64, a.kv_heads, 1);
+}
+
+// Forward and dq: the most row sets that still make two workgroups for every
+// CU.  us of the forward pass in 4, 2 and 1 sets (MI355X): bf16, heads x rows of
+// 32 x 4096 x 128 156, 180, 454; 32 x 1400 x 64 28, 22, 33; 8 x 1000 x 64 21, 16,
+// 12; fp32, 32 x 1500 x 64 137, 100, 137; 8 x 1000 x 64 77, 43, 28.
+template <typename T, int DP, typename F>
+void packed_by_sets(const PackedArgs& a, F f) {
+    constexpr int FEW = packed_few_sets<T, DP>();
+    if (packed_enough(a, 128, a.heads, 2)) return f.template sets<T, DP, 4>();
+    if constexpr (FEW < 2) {
+        if (packed_enough(a, 64, a.heads, 2)) return f.template sets<T, DP, 2>();
+    }
+    f.template sets<T, DP, FEW>();
 }
 
 // f.run<T, DP>() for a type and a head size

@@ -1,10 +1,12 @@
 // rac_packed_dkv.hip — packed causal attention, the gradients of k and v.
 #include "rac_packed.hpp"
+#include <type_traits>
 
 namespace rac {
 
 // WHICH: 1 dv, 2 dk, 3 both (d past 128 in fp32 has no registers for both)
-template <typename T, int DP, int WR, int WHICH>
+// BY_HEAD: a workgroup sums one query head's part, in fp32, for the join below
+template <typename T, int DP, int WR, int WHICH, bool BY_HEAD>
 __global__ __launch_bounds__(kPkThreads, DP * sizeof(T) <= 128 ? 2 : 1) void packed_dkv_kernel(const PackedArgs a) {
     using M = Mma<T>;
     using Frag = typename M::Frag;
@@ -14,30 +16,33 @@ __global__ __launch_bounds__(kPkThreads, DP * sizeof(T) <= 128 ? 2 : 1) void pac
     constexpr bool WV = WHICH & 1, WK = WHICH & 2;
     __shared__ __attribute__((aligned(16))) char qa[S::BYTES], ga[S::BYTES], qb[S::BYTES], gb[S::BYTES];
     __shared__ __attribute__((aligned(16))) float sa[2 * TILE], sb[2 * TILE];       // log2 sums and D
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), half = lane >> 5;
+    const int lane0 = threadIdx.x & 63, lane = lane0, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), half = lane >> 5;
     const int wr = wave % WR, kg = wave / WR;
-    int g, tile;
-    packed_block(a.kv_heads, g, tile);
+    using O = typename std::conditional<BY_HEAD, float, T>::type;
+    int h, tile;
+    packed_block(BY_HEAD ? a.heads : a.kv_heads, h, tile);
+    const int group = a.heads / a.kv_heads, g = BY_HEAD ? h / group : h;
     const PackedSeg seg = packed_tile(a.cu, a.n_seqs, a.total, tile, S::ROWS, true);
     if (seg.kind == 0) return;
-    T* dk = (T*)a.dk;
-    T* dv = (T*)a.dv;
+    O* dk = BY_HEAD ? (O*)a.part : (O*)a.dk;
+    O* dv = BY_HEAD ? (O*)(a.part + (long)a.total * a.heads * a.d) : (O*)a.dv;
     if (seg.kind == 2) {
         const int rows = min(S::ROWS, seg.len - seg.row0);
-        if (a.zero_rest) {
+        if (!BY_HEAD && a.zero_rest) {
             if (WK) packed_zero(dk, seg.start + seg.row0, rows, a.kv_heads, g, a.d);
             if (WV) packed_zero(dv, seg.start + seg.row0, rows, a.kv_heads, g, a.d);
         }
         return;
     }
     const int k0 = seg.row0, kw = k0 + 32 * wr, key = kw + (lane & 31);
-    const int rep = a.heads / a.kv_heads;
+    const int rep = BY_HEAD ? 1 : group, h0 = BY_HEAD ? h : g * group;      // query heads of the sum
+    const int oheads = BY_HEAD ? a.heads : a.kv_heads;
     const bool there = key < seg.len;
     const long row = seg.start + key;
     // steps: the tiles of queries from the diagonal on, for one head of the group after the other
     const int t0 = k0 / TILE, per = (seg.len + TILE - 1) / TILE - t0, steps = per * rep;
-    const T* const Q = (const T*)a.q + (long)seg.start * a.sq_t + (long)g * rep * a.sq_h;
-    const T* const G = (const T*)a.grad + ((long)seg.start * a.heads + (long)g * rep) * a.d;
+    const T* const Q = (const T*)a.q + (long)seg.start * a.sq_t + (long)h0 * a.sq_h;
+    const T* const G = (const T*)a.grad + ((long)seg.start * a.heads + h0) * a.d;
     // direct also in 16 bits: 6 bf16 documents of 8192 rows (32/8 heads of 128)
     // 795 us, through registers 870
     TileLoad<T, DP, TILE, true> lq, lg;
@@ -51,7 +56,7 @@ __global__ __launch_bounds__(kPkThreads, DP * sizeof(T) <= 128 ? 2 : 1) void pac
         lq.issue(qd, Q + (long)ih * a.sq_h + (long)first * a.sq_t, left, a.sq_t, a.d, a.vec, wave);
         lg.issue(gd, G + (long)ih * a.d + (long)first * a.heads * a.d, left, (long)a.heads * a.d, a.d, a.vec, wave);
         if (slot < 2 * TILE) {
-            const float* base = a.stats + 2 * ((long)(g * rep + ih) * a.total + seg.start + first);
+            const float* base = a.stats + 2 * ((long)(h0 + ih) * a.total + seg.start + first);
             // rows past the sequence: 0, next to zeros of do no matter
             stat_next = slot < 2 * left ? base[slot] : 0.0f;
         }
@@ -80,6 +85,8 @@ __global__ __launch_bounds__(kPkThreads, DP * sizeof(T) <= 128 ? 2 : 1) void pac
     }
     int ct = t0;                                          // tile of this step
     auto work = [&](const char* qs, const char* gs, const float* ss) ATTN_INLINE {
+        // rows this long fill the registers: no tile's address stays in one
+        const int lane = DP * sizeof(T) >= 512 ? attn_fresh(lane0) : lane0, half = lane >> 5;
         const int first = ct * TILE + kg * BQ, row0 = kg * BQ;
         if (++ct == t0 + per) ct = t0;
         auto scores = [&](int u, f32x16& s, f32x16& dp) ATTN_INLINE {
@@ -118,32 +125,24 @@ __global__ __launch_bounds__(kPkThreads, DP * sizeof(T) <= 128 ? 2 : 1) void pac
                 }
             }
         };
-        if (first >= kw + 31) {
-            // every query sees every key of the wave
-            f32x16 s[NS], dp[NS];
-#pragma unroll
-            for (int u = 0; u < NS; u++) scores(u, s[u], dp[u]);
-#pragma unroll
-            for (int u = 0; u < NS; u++) {
-                weights(u, s[u], dp[u]);
-                sums(u, s[u], dp[u]);
-            }
-            return;
-        }
-#pragma unroll 1
-        for (int u = 0; u < NS; u++) {
-            const int q0 = first + 32 * u;
-            if (q0 + 31 < kw || q0 >= seg.len) continue;     // before the wave's keys, or past the sequence
-            f32x16 s, dp;
-            scores(u, s, dp);
-            weights(u, s, dp);
+        auto mask = [&](int q0, f32x16& s, f32x16& dp) ATTN_INLINE {
+            attn_branch();
 #pragma unroll
             for (int i = 0; i < 16; i++)
-                if (q0 + 8 * (i / 4) + 4 * half + i % 4 < key) {
+                if (q0 + 8 * (i / 4) + 4 * half + i % 4 < kw + (lane & 31)) {
                     s[i] = 0.0f;
                     if constexpr (WK) dp[i] = 0.0f;
                 }
-            sums(u, s, dp);
+        };
+        if (first + BQ - 1 < kw || first >= seg.len) return;      // before the wave's keys, or past the sequence
+        f32x16 s[NS], dp[NS];
+#pragma unroll
+        for (int u = 0; u < NS; u++) scores(u, s[u], dp[u]);
+#pragma unroll
+        for (int u = 0; u < NS; u++) {
+            weights(u, s[u], dp[u]);
+            if (first + 32 * u < kw + 31) mask(first + 32 * u, s[u], dp[u]);
+            sums(u, s[u], dp[u]);
         }
     };
     auto step = [&](int st, const char* qs, const char* gs, const float* ss, char* qn, char* gn, float* sn) ATTN_INLINE {
@@ -168,19 +167,19 @@ __global__ __launch_bounds__(kPkThreads, DP * sizeof(T) <= 128 ? 2 : 1) void pac
     uint64_t again = __ballot(bad && there);
     again = (again | again >> 32) & 0xffffffffull;
     if (there && !(again >> (lane & 31) & 1)) {
-        const long at = (row * a.kv_heads + g) * a.d;
-        if constexpr (WK) attn_store<T, ND>(dk + at, ak, a.scale, a.d, half, a.vec_out);
-        if constexpr (WV) attn_store<T, ND>(dv + at, av, 1.0f, a.d, half, a.vec_out);
+        const long at = (row * oheads + h) * a.d;
+        if constexpr (WK) attn_store<O, ND>(dk + at, ak, a.scale, a.d, half, BY_HEAD ? a.d % 4 == 0 : a.vec_out);
+        if constexpr (WV) attn_store<O, ND>(dv + at, av, 1.0f, a.d, half, BY_HEAD ? a.d % 4 == 0 : a.vec_out);
     }
     for (; again; again &= again - 1) {
         const int kr = kw + __ffsll((unsigned long long)again) - 1, from = kr, n = seg.len - from;
-        const long at = ((long)(seg.start + kr) * a.kv_heads + g) * a.d;
+        const long at = ((long)(seg.start + kr) * oheads + h) * a.d;
         const T* kk = (const T*)a.k + (long)(seg.start + kr) * a.sk_t + (long)g * a.sk_h;
         const T* vv = (const T*)a.v + (long)(seg.start + kr) * a.sv_t + (long)g * a.sv_h;
         // queries from .. of head 0 of the group, then of head 1, ...
         auto qrow = [&](int i) { return Q + (long)(i / n) * a.sq_h + (long)(from + i % n) * a.sq_t; };
         auto grow = [&](int i) { return G + ((long)(from + i % n) * a.heads + i / n) * a.d; };
-        auto stats_of = [&](int i) { return a.stats + 2 * ((long)(g * rep + i / n) * a.total + seg.start + from + i % n); };
+        auto stats_of = [&](int i) { return a.stats + 2 * ((long)(h0 + i / n) * a.total + seg.start + from + i % n); };
         auto prob = [&](int i) { return exp2_hw(__builtin_fmaf(row_dot(qrow(i), kk, a.d), c, -*stats_of(i))); };
         if constexpr (WV) attn_again<T, DP>(dv + at, 1.0f, a.d, 0, n * rep, prob, grow);
         if constexpr (WK)
@@ -189,29 +188,75 @@ __global__ __launch_bounds__(kPkThreads, DP * sizeof(T) <= 128 ? 2 : 1) void pac
     }
 }
 
+// dk and dv from their query heads' parts, in the order of the heads: a thread
+// per value.
+template <typename T>
+__global__ __launch_bounds__(kPkThreads) void packed_join_kernel(const PackedArgs a) {
+    const int rep = a.heads / a.kv_heads;
+    const long i = (long)blockIdx.x * kPkThreads + threadIdx.x;
+    if (i >= (long)a.total * a.kv_heads * a.d) return;
+    const int row = (int)(i / ((long)a.kv_heads * a.d)), c = (int)(i % a.d), g = (int)(i / a.d % a.kv_heads);
+    const int first = min(max(a.cu[0], 0), a.total), end = min(max(a.cu[a.n_seqs], first), a.total);
+    const bool in = row >= first && row < end;
+    if (!in && !a.zero_rest) return;
+    float k = 0.0f, v = 0.0f;
+    if (in) {
+        const float* pk = a.part + ((long)row * a.heads + (long)g * rep) * a.d + c;
+        const float* pv = pk + (long)a.total * a.heads * a.d;
+        for (int r = 0; r < rep; r++) {
+            k += pk[(long)r * a.d];
+            v += pv[(long)r * a.d];
+        }
+    }
+    ((T*)a.dk)[i] = Mma<T>::from_f32(k);
+    ((T*)a.dv)[i] = Mma<T>::from_f32(v);
+}
+
 // ── launch ──────────────────────────────────────────────────────────────
 
 namespace {
 struct Launch {
     const PackedArgs& a;
     hipStream_t s;
-    template <typename T, int DP, int WR>
+    template <typename T, int DP, int WR, bool BY_HEAD>
     void sets() const {
-        const dim3 grid((unsigned)(packed_tiles(a, 32 * WR) * a.kv_heads)), t(kPkThreads);
-        if constexpr (DP * sizeof(T) > 512) {
-            hipLaunchKernelGGL((packed_dkv_kernel<T, DP, WR, 1>), grid, t, 0, s, a);
-            hipLaunchKernelGGL((packed_dkv_kernel<T, DP, WR, 2>), grid, t, 0, s, a);
+        const dim3 grid((unsigned)(packed_tiles(a, 32 * WR) * (BY_HEAD ? a.heads : a.kv_heads))), t(kPkThreads);
+        if constexpr (DP == 256) {
+            hipLaunchKernelGGL((packed_dkv_kernel<T, DP, WR, 1, BY_HEAD>), grid, t, 0, s, a);
+            hipLaunchKernelGGL((packed_dkv_kernel<T, DP, WR, 2, BY_HEAD>), grid, t, 0, s, a);
         } else {
-            hipLaunchKernelGGL((packed_dkv_kernel<T, DP, WR, 3>), grid, t, 0, s, a);
+            hipLaunchKernelGGL((packed_dkv_kernel<T, DP, WR, 3, BY_HEAD>), grid, t, 0, s, a);
         }
+    }
+    // The most row sets that still make a workgroup for every CU, in 16 bits two
+    // at most and in rows of 64 bytes one: shorter tiles even out the triangle.
+    // us of the backward pass in 4, 2 and 1 sets (MI355X): 6 bf16 documents of
+    // 8192 rows, 32/8 heads of 128, 949, 819, 1420; 64 532, 430, 444; 32 372, 293,
+    // 255; one of 8192, 32/4 heads of 128, 3497, 2327, 3949.
+    template <typename T, int DP, bool BY_HEAD>
+    void run_heads() const {
+        constexpr int FEW = packed_few_sets<T, DP>();
+        const int heads = BY_HEAD ? a.heads : a.kv_heads;
+        if constexpr (sizeof(T) == 4 || DP == 256) {
+            if (packed_enough(a, 128, heads, 1)) return sets<T, DP, 4, BY_HEAD>();
+        }
+        if constexpr (FEW < 2 && DP > 32) {
+            if (packed_enough(a, 64, heads, 1)) return sets<T, DP, 2, BY_HEAD>();
+        }
+        sets<T, DP, FEW, BY_HEAD>();
     }
     template <typename T, int DP>
     void run() const {
-        if (packed_few(a, a.kv_heads)) sets<T, DP, packed_few_sets<T, DP>()>();
-        else sets<T, DP, 4>();
+        if (!packed_by_head_parts(a)) return run_heads<T, DP, false>();
+        run_heads<T, DP, true>();
+        const long n = (long)a.total * a.kv_heads * a.d;
+        hipLaunchKernelGGL((packed_join_kernel<T>), dim3((unsigned)((n + kPkThreads - 1) / kPkThreads)), dim3(kPkThreads), 0,
+                           s, a);
     }
 };
 }  // namespace
+
+long packed_dkv_parts(const PackedArgs& a) { return packed_by_head_parts(a) ? 2L * a.total * a.heads * a.d : 0; }
 
 hipError_t packed_dkv_launch(const PackedArgs& a, int dtype, hipStream_t s) {
     packed_by_type(dtype, a.d, Launch{a, s});

@@ -11,7 +11,7 @@ __global__ __launch_bounds__(kPkThreads, DP * sizeof(T) <= 256 ? 2 : 1) void pac
     using TL = Tile<T, DP>;
     constexpr int KG = S::KG, BN = S::BN, TILE = S::TILE, ND = S::ND, NF = S::NF, NS = S::NS, FS = S::FS;
     __shared__ __attribute__((aligned(16))) char ka[S::BYTES], va[S::BYTES], kb[S::BYTES], vb[S::BYTES];
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), half = lane >> 5;
+    const int lane0 = threadIdx.x & 63, lane = lane0, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), half = lane >> 5;
     const int wr = wave % WR, kg = wave / WR;
     int h, tile;
     packed_block(a.heads, h, tile);
@@ -70,6 +70,8 @@ __global__ __launch_bounds__(kPkThreads, DP * sizeof(T) <= 256 ? 2 : 1) void pac
     for (int n = 0; n < ND; n++) acc[n] = zero16();
 
     auto work = [&](int j, const char* ks, const char* vs) ATTN_INLINE {
+        // rows this long fill the registers: no tile's address stays in one
+        const int lane = DP * sizeof(T) >= 1024 ? attn_fresh(lane0) : lane0, half = lane >> 5;
         const int first = j * TILE + kg * BN;
         if (first > qw + 31) return;
         const bool diag = first + BN - 1 > qw;
@@ -148,8 +150,7 @@ struct Launch {
     }
     template <typename T, int DP>
     void run() const {
-        if (packed_few(a, a.heads)) sets<T, DP, packed_few_sets<T, DP>()>();
-        else sets<T, DP, 4>();
+        packed_by_sets<T, DP>(a, *this);
     }
 };
 }  // namespace

@@ -1194,8 +1194,8 @@ def packed_attention_backward(grad_out: torch.Tensor, q: torch.Tensor, k: torch.
     dk, dv = (torch.empty(k.shape, device=q.device, dtype=q.dtype) for _ in range(2))
     scale = _default_scale(D) if scale is None else float(scale)
     if total:
-        ws = torch.empty(_lib.load().rac_packed_attention_backward_workspace_bytes(total, H) // 4, device=q.device,
-                         dtype=torch.float32)
+        n = _lib.load().rac_packed_attention_backward_workspace_bytes(cu.numel() - 1, total, H, k.size(1), D)
+        ws = torch.empty(n // 4, device=q.device, dtype=torch.float32)
         _call("rac_packed_attention_backward_dev", q, q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(),
               grad_out.data_ptr(), lse.data_ptr(), cu.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(),
               ws.data_ptr(), cu.numel() - 1, total, H, k.size(1), D, *_packed_tail(q, k, v), scale, 1, dt)

@@ -109,8 +109,10 @@ def test_nothing_to_do_is_no_error(lib):
 
 
 def test_workspace_sizes(lib):
-    assert lib.rac_packed_attention_backward_workspace_bytes(100, 8) == 6400
-    assert lib.rac_packed_attention_backward_workspace_bytes(0, 8) == 0
+    size = lib.rac_packed_attention_backward_workspace_bytes
+    assert size(3, 100, 8, 8, 64) == 6400 and size(1, 0, 8, 8, 64) == 0 and size(1, 100, 8, 3, 64) == 0
+    assert size(3, 101, 3, 3, 64) == 4 * 608                # the statistics, up to 16 bytes
+    assert size(3, 100, 8, 2, 64) >= 6400
     assert lib.rac_tree_attention_workspace_bytes(0, 4, 4, 2, 64, 100, 0) == 0
     assert lib.rac_tree_attention_workspace_bytes(1, 300, 4, 2, 64, 1000, 0) == 0
     assert lib.rac_token_logprobs_workspace_bytes(0, 100, 0, 0) == 0
