@@ -36,25 +36,29 @@ extern "C" {
  * d_head] with element strides per row and per head; query head h reads key /
  * value head h / (n_heads / n_kv_heads).  out[t, h] = sum_{j <= t} p_j v_j,
  * p = softmax(scale q_t . k_j), contiguous [total, n_heads, d_head]; lse
- * [n_heads, total] (may be null) receives log sum_j exp(scale q_t . k_j).
+ * [n_heads, total] (may be null) receives log sum_j exp(scale q_t . k_j), out_lo
+ * (out's shape and type, may be null; the 16-bit types) what the rounding of out
+ * took away, for the backward pass.
  * Rows of out outside every sequence become 0 with zero_rest and stay as they
  * are without; their lse stays as it is.  A row whose scores are all -inf gives
  * 0; values at positions a row does not see never reach it, NaN included.
  * scale > 0; total <= 2^30. */
-int rac_packed_attention_dev(const void *q, const void *k, const void *v, void *out, float *lse,
+int rac_packed_attention_dev(const void *q, const void *k, const void *v, void *out, void *out_lo, float *lse,
                              const int *cu_seqlens, int n_seqs, int total, int n_heads, int n_kv_heads, int d_head,
                              long q_stride, long q_head_stride, long k_stride, long k_head_stride, long v_stride,
                              long v_head_stride, float scale, int zero_rest, int dtype, void *stream);
 
 /* Its gradients: grad_out, out, dq [total, n_heads, d_head], dk and dv [total,
- * n_kv_heads, d_head] contiguous, lse as the forward pass left it.  dk and dv
+ * n_kv_heads, d_head] contiguous, lse and out_lo (may
+ * be null: the gradients of q and k are then about half again as far off in the
+ * 16-bit types) as the forward pass left them.  dk and dv
  * are sums over the query heads that share a head, taken in a fixed order: the
  * same call gives the same bits.  workspace:
  * rac_packed_attention_backward_workspace_bytes bytes on a 16-byte boundary, the
  * call's own while it runs. */
 long rac_packed_attention_backward_workspace_bytes(int n_seqs, int total, int n_heads, int n_kv_heads, int d_head);
 int rac_packed_attention_backward_dev(const void *q, const void *k, const void *v, const void *out,
-                                      const void *grad_out, const float *lse, const int *cu_seqlens, void *dq,
+                                      const void *out_lo, const void *grad_out, const float *lse, const int *cu_seqlens, void *dq,
                                       void *dk, void *dv, float *workspace, int n_seqs, int total, int n_heads,
                                       int n_kv_heads, int d_head, long q_stride, long q_head_stride, long k_stride,
                                       long k_head_stride, long v_stride, long v_head_stride, float scale,

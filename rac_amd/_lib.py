@@ -105,9 +105,9 @@ _SIGNATURES = {
     "rac_decode_qkv_dev": (_i, [_vp, _vp, _f, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _l, _vp, _vp]),
     "rac_decode_swiglu_gemv_dev": (_i, [_vp, _vp, _f, _vp, _vp, _i, _i, _i, _vp]),
     # rac_llm.h — packed prompts, drafted tokens, given tokens
-    "rac_packed_attention_dev": (_i, [_vp] * 6 + [_i] * 5 + [_l] * 6 + [_f, _i, _i, _vp]),
+    "rac_packed_attention_dev": (_i, [_vp] * 7 + [_i] * 5 + [_l] * 6 + [_f, _i, _i, _vp]),
     "rac_packed_attention_backward_workspace_bytes": (_l, [_i] * 5),
-    "rac_packed_attention_backward_dev": (_i, [_vp] * 11 + [_i] * 5 + [_l] * 6 + [_f, _i, _i, _vp]),
+    "rac_packed_attention_backward_dev": (_i, [_vp] * 12 + [_i] * 5 + [_l] * 6 + [_f, _i, _i, _vp]),
     "rac_tree_attention_workspace_bytes": (_l, [_i] * 5 + [_l, _i]),
     "rac_tree_attention_dev": (_i, [_vp] * 7 + [_i] * 5 + [_l] * 11 + [_f, _i, _vp]),
     "rac_token_logprobs_workspace_bytes": (_l, [_l, _l, _i, _i]),

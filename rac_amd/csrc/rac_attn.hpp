@@ -178,6 +178,24 @@ __device__ __forceinline__ void load_frags(typename Mma<T>::Frag (&fr)[DP / Mma<
                                    there ? load_chunk(row, f * KF + half * (KF / 2), d, vec) : u32x4{0, 0, 0, 0});
 }
 
+// 4 values at columns c .. of a row
+template <typename T>
+__device__ __forceinline__ void store4(T* row, int c, const float (&v)[4], int d, bool vec) {
+    union { T e[4]; u32x2 v2; u32x4 v4; } u;
+#pragma unroll
+    for (int j = 0; j < 4; j++) u.e[j] = Mma<T>::from_f32(v[j]);
+    if (vec) {
+        if (c < d) {
+            if constexpr (sizeof(T) == 2) *reinterpret_cast<u32x2*>(row + c) = u.v2;
+            else *reinterpret_cast<u32x4*>(row + c) = u.v4;
+        }
+    } else {
+#pragma unroll
+        for (int j = 0; j < 4; j++)
+            if (c + j < d) row[c + j] = u.e[j];
+    }
+}
+
 // a 32-column accumulator set (DP rows of d) times f into one contiguous row
 template <typename T, int ND>
 __device__ __forceinline__ void attn_store(T* row, const f32x16 (&acc)[ND], float f, int d, int half, bool vec) {
@@ -185,20 +203,26 @@ __device__ __forceinline__ void attn_store(T* row, const f32x16 (&acc)[ND], floa
     for (int n = 0; n < ND; n++)
 #pragma unroll
         for (int b = 0; b < 4; b++) {
-            const int c = 32 * n + 8 * b + 4 * half;
-            union { T e[4]; u32x2 v2; u32x4 v4; } u;
+            float v[4];
 #pragma unroll
-            for (int j = 0; j < 4; j++) u.e[j] = Mma<T>::from_f32(acc[n][4 * b + j] * f);
-            if (vec) {
-                if (c < d) {
-                    if constexpr (sizeof(T) == 2) *reinterpret_cast<u32x2*>(row + c) = u.v2;
-                    else *reinterpret_cast<u32x4*>(row + c) = u.v4;
-                }
-            } else {
+            for (int j = 0; j < 4; j++) v[j] = acc[n][4 * b + j] * f;
+            store4(row, 32 * n + 8 * b + 4 * half, v, d, vec);
+        }
+}
+// what the rounding to T took from that
+template <typename T, int ND>
+__device__ __forceinline__ void attn_store_rest(T* row, const f32x16 (&acc)[ND], float f, int d, int half, bool vec) {
 #pragma unroll
-                for (int j = 0; j < 4; j++)
-                    if (c + j < d) row[c + j] = u.e[j];
+    for (int n = 0; n < ND; n++)
+#pragma unroll
+        for (int b = 0; b < 4; b++) {
+            float v[4];
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                v[j] = acc[n][4 * b + j] * f;
+                v[j] -= Mma<T>::to_f32(Mma<T>::from_f32(v[j]));
             }
+            store4(row, 32 * n + 8 * b + 4 * half, v, d, vec);
         }
 }
 
@@ -233,7 +257,7 @@ __device__ void row_axpy(float (&acc)[(DP + 63) / 64], float f, const T* y, int 
 // one to a lane, then their rows one by one; nothing of a j outside is read
 // (with SKIP, nor of a j whose weight is below 0)
 template <typename T, int DP, bool SKIP = false, typename O, typename W, typename R>
-__device__ void attn_again(O* out, float f, int d, int j0, int j1, W w, R rows) {
+__device__ void attn_again(O* out, float f, int d, int j0, int j1, W w, R rows, O* lo = nullptr) {
     float acc[(DP + 63) / 64] = {};
     for (int j = j0; j < j1; j += 64) {
         const int mine = j + (threadIdx.x & 63);
@@ -246,7 +270,11 @@ __device__ void attn_again(O* out, float f, int d, int j0, int j1, W w, R rows) 
 #pragma unroll
     for (int n = 0; n < (DP + 63) / 64; n++) {
         const int c = (threadIdx.x & 63) + 64 * n;
-        if (c < d) out[c] = Mma<O>::from_f32(acc[n] * f);
+        if (c < d) {
+            const float v = acc[n] * f;
+            out[c] = Mma<O>::from_f32(v);
+            if (lo) lo[c] = Mma<O>::from_f32(v - Mma<O>::to_f32(out[c]));
+        }
     }
 }
 

@@ -505,20 +505,20 @@ static int packed_args(const char* who, PackedArgs* a, int dtype) {
     return RAC_OK;
 }
 
-RAC_EXPORT int rac_packed_attention_dev(const void* q, const void* k, const void* v, void* out, float* lse,
+RAC_EXPORT int rac_packed_attention_dev(const void* q, const void* k, const void* v, void* out, void* out_lo, float* lse,
                                         const int* cu_seqlens, int n_seqs, int total, int n_heads, int n_kv_heads,
                                         int d_head, long q_stride, long q_head_stride, long k_stride,
                                         long k_head_stride, long v_stride, long v_head_stride, float scale,
                                         int zero_rest, int dtype, void* stream) {
     const char* who = "rac_packed_attention_dev";
     if (!q || !k || !v || !out || !cu_seqlens) return fail(RAC_ERR_NULL_PTR, "%s: null buffer", who);
-    PackedArgs a{q, k, v, nullptr, out, nullptr, nullptr, nullptr, lse, nullptr, nullptr, cu_seqlens, n_seqs, total, n_heads,
+    PackedArgs a{q, k, v, nullptr, out, out_lo, nullptr, nullptr, nullptr, lse, nullptr, nullptr, cu_seqlens, n_seqs, total, n_heads,
                  n_kv_heads, d_head, q_stride, q_head_stride, k_stride, k_head_stride, v_stride, v_head_stride, scale,
                  zero_rest, false, false};
     const int rc = packed_args(who, &a, dtype);
     if (rc) return rc;
     const int es = dtype == 0 ? 4 : 2;
-    a.vec_out = (uintptr_t)out % (4 * es) == 0 && d_head % 4 == 0;
+    a.vec_out = ((uintptr_t)out | (uintptr_t)out_lo) % (4 * es) == 0 && d_head % 4 == 0;
     if (total == 0) return RAC_OK;
     return check_hip(packed_fwd_launch(a, dtype, (hipStream_t)stream), "rac_packed_attention_dev launch");
 }
@@ -538,7 +538,7 @@ RAC_EXPORT long rac_packed_attention_backward_workspace_bytes(int n_seqs, int to
 }
 
 RAC_EXPORT int rac_packed_attention_backward_dev(const void* q, const void* k, const void* v, const void* out,
-                                                 const void* grad_out, const float* lse, const int* cu_seqlens,
+                                                 const void* out_lo, const void* grad_out, const float* lse, const int* cu_seqlens,
                                                  void* dq, void* dk, void* dv, float* workspace, int n_seqs, int total,
                                                  int n_heads, int n_kv_heads, int d_head, long q_stride,
                                                  long q_head_stride, long k_stride, long k_head_stride, long v_stride,
@@ -547,14 +547,15 @@ RAC_EXPORT int rac_packed_attention_backward_dev(const void* q, const void* k, c
     const char* who = "rac_packed_attention_backward_dev";
     if (!q || !k || !v || !out || !grad_out || !lse || !cu_seqlens || !dq || !dk || !dv || !workspace)
         return fail(RAC_ERR_NULL_PTR, "%s: null buffer", who);
-    PackedArgs a{q, k, v, grad_out, const_cast<void*>(out), dq, dk, dv, const_cast<float*>(lse), workspace,
+    PackedArgs a{q, k, v, grad_out, const_cast<void*>(out), const_cast<void*>(out_lo), dq, dk, dv, const_cast<float*>(lse), workspace,
                  workspace + (2L * total * n_heads + 3) / 4 * 4, cu_seqlens,
                  n_seqs, total, n_heads, n_kv_heads, d_head, q_stride, q_head_stride, k_stride, k_head_stride, v_stride,
                  v_head_stride, scale, zero_rest, false, false};
     const int rc = packed_args(who, &a, dtype);
     if (rc) return rc;
     const int es = dtype == 0 ? 4 : 2;
-    a.vec = a.vec && rows_aligned(out, es, d_head, 0, 0) && rows_aligned(grad_out, es, d_head, 0, 0);
+    a.vec = a.vec && rows_aligned(out, es, d_head, 0, 0) && rows_aligned(out_lo, es, d_head, 0, 0) &&
+            rows_aligned(grad_out, es, d_head, 0, 0);
     a.vec_out = ((uintptr_t)dq | (uintptr_t)dk | (uintptr_t)dv) % (4 * es) == 0 && d_head % 4 == 0;
     if (total == 0) return RAC_OK;
     hipError_t e = packed_dq_launch(a, dtype, (hipStream_t)stream);

@@ -186,7 +186,7 @@ hipError_t swiglu_launch(const float* gu, float* out, long n, int iters, hipStre
 // Causal attention over packed sequences (rac_packed.hip): q [total, heads, d],
 // k and v [total, kv_heads, d] with element strides per row (_t) and head (_h);
 // out, grad, dq [total, heads, d], dk, dv [total, kv_heads, d] contiguous; lse
-// [heads, total]; stats [heads, total, 2]: log2 of the sums (of rows without any:
+// [heads, total]; out_lo (may be null): what rounding took from a 16-bit out; stats [heads, total, 2]: log2 of the sums (of rows without any:
 // +inf) and D = do . o; part: dk and dv of every query head in fp32, each [total,
 // heads, d] (null: packed_dkv_parts is 0).  vec: every row of q, k, v (and out, grad in a backward
 // pass) is 16-byte aligned and d whole 16-byte vectors; vec_out: the outputs'
@@ -195,7 +195,7 @@ hipError_t swiglu_launch(const float* gu, float* out, long n, int iters, hipStre
 constexpr int kPackedMaxHead = 256;
 struct PackedArgs {
     const void *q, *k, *v, *grad;
-    void *out, *dq, *dk, *dv;
+    void *out, *out_lo, *dq, *dk, *dv;
     float *lse, *stats, *part;
     const int* cu;
     int n_seqs, total, heads, kv_heads, d;

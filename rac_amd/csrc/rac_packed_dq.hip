@@ -42,20 +42,30 @@ __global__ __launch_bounds__(kPkThreads, DP * sizeof(T) <= 256 ? 2 : 1) void pac
         lk.commit(kd, K + (long)j * TILE * a.sk_t, seg.len - j * TILE, a.sk_t, a.d, a.vec);
         lv.commit(vd, V + (long)j * TILE * a.sv_t, seg.len - j * TILE, a.sv_t, a.d, a.vec);
     };
+    // D = do . o, kept for the keys' kernel beside the log sums.  A rounded o
+    // alone would leave D, and through it every ds of the row, off by as much as
+    // all their own roundings together: what its rounding took is added.
+    float dl = 0.0f;
+    if (there) {
+        const long at = (row * a.heads + h) * a.d;
+#pragma unroll 4
+        for (int f = 0; f < NF; f++) {
+            const int at_f = f * M::KF + half * (M::KF / 2);
+            auto chunk = [&](const void* p) ATTN_INLINE {
+                return __builtin_bit_cast(Frag, load_chunk((const T*)p + at, at_f, a.d, a.vec));
+            };
+            const Frag go = chunk(a.grad), of = chunk(a.out), lo = sizeof(T) == 2 && a.out_lo ? chunk(a.out_lo) : Frag{};
+#pragma unroll
+            for (int e = 0; e < M::VEC; e++) {
+                dl = __builtin_fmaf(M::to_f32(go[e]), M::to_f32(of[e]), dl);
+                if (sizeof(T) == 2) dl = __builtin_fmaf(M::to_f32(go[e]), M::to_f32(lo[e]), dl);
+            }
+        }
+    }
     issue(0, ka, va);
     Frag qf[NF], gf[NF];
     load_frags<T, DP>(qf, (const T*)a.q + row * a.sq_t + (long)h * a.sq_h, there, a.d, half, a.vec);
     load_frags<T, DP>(gf, (const T*)a.grad + (row * a.heads + h) * a.d, there, a.d, half, a.vec);
-    // D = do . o, kept for the keys' kernel beside the log sums
-    float dl = 0.0f;
-    {
-        Frag of[NF];
-        load_frags<T, DP>(of, (const T*)a.out + (row * a.heads + h) * a.d, there, a.d, half, a.vec);
-#pragma unroll
-        for (int f = 0; f < NF; f++)
-#pragma unroll
-            for (int e = 0; e < M::VEC; e++) dl = __builtin_fmaf(M::to_f32(gf[f][e]), M::to_f32(of[f][e]), dl);
-    }
     dl = half_sum(dl);
     // rows without a key that counts (lse -inf) and rows past the sequence: p = 0
     float lse = there ? a.lse[(long)h * a.total + row] * kLog2e : __builtin_inff();

@@ -19,6 +19,7 @@ __global__ __launch_bounds__(kPkThreads, DP * sizeof(T) <= 256 ? 2 : 1) void pac
     const PackedSeg seg = packed_tile(a.cu, a.n_seqs, a.total, tile, S::ROWS, false);
     if (seg.kind == 0) return;
     T* out = (T*)a.out;
+    T* lo = (T*)a.out_lo;
     if (seg.kind == 2) {
         if (a.zero_rest) packed_zero(out, seg.start + seg.row0, min(S::ROWS, seg.len - seg.row0), a.heads, h, a.d);
         return;
@@ -144,16 +145,21 @@ __global__ __launch_bounds__(kPkThreads, DP * sizeof(T) <= 256 ? 2 : 1) void pac
     again = (again | again >> 32) & 0xffffffffull;
     if (qrow < seg.len) {
         const long row = seg.start + qrow;
-        if (!(again >> (lane & 31) & 1)) attn_store<T, ND>(out + (row * a.heads + h) * a.d, o, inv, a.d, half, a.vec_out);
+        const long at = (row * a.heads + h) * a.d;
+        if (!(again >> (lane & 31) & 1)) {
+            attn_store<T, ND>(out + at, o, inv, a.d, half, a.vec_out);
+            if (sizeof(T) == 2 && lo) attn_store_rest<T, ND>(lo + at, o, inv, a.d, half, a.vec_out);
+        }
         if (a.lse && half == 0) a.lse[(long)h * a.total + row] = (m + __builtin_amdgcn_logf(l)) * kLn2;
     }
     for (; again; again &= again - 1) {
         const int r = __ffsll((unsigned long long)again) - 1, t = qw + r;
         const float mr = __shfl(m, r), ir = __shfl(inv, r);
         const T* q = (const T*)a.q + (long)(seg.start + t) * a.sq_t + (long)h * a.sq_h;
-        attn_again<T, DP>(out + ((long)(seg.start + t) * a.heads + h) * a.d, ir, a.d, 0, t + 1,
+        const long at = ((long)(seg.start + t) * a.heads + h) * a.d;
+        attn_again<T, DP>(out + at, ir, a.d, 0, t + 1,
                           [&](int j) { return exp2_hw(__builtin_fmaf(row_dot(q, K + (long)j * a.sk_t, a.d), c, -mr)); },
-                          [&](int j) { return V + (long)j * a.sv_t; });
+                          [&](int j) { return V + (long)j * a.sv_t; }, lo && sizeof(T) == 2 ? lo + at : nullptr);
     }
 }
 

@@ -1149,7 +1149,8 @@ def _packed_tail(q, k, v):
 
 
 def packed_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqlens: torch.Tensor,
-                     scale: Optional[float] = None, return_lse: bool = False, out: Optional[torch.Tensor] = None):
+                     scale: Optional[float] = None, return_lse: bool = False, out: Optional[torch.Tensor] = None,
+                     return_residual: bool = False):
     """Causal attention within each of several sequences packed one behind
     the other: sequence i is rows cu_seqlens[i] .. cu_seqlens[i + 1] - 1
     (int32, on the device, non-decreasing; sequences may be empty) of q
@@ -1158,31 +1159,39 @@ def packed_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqle
     (slices of a stacked projection).  Query head h reads key / value head
     h // (n_heads / n_kv_heads); scale defaults to 1 / sqrt(d_head).  Returns
     [total, n_heads, d_head]; with return_lse also log sum exp of the scores
-    [n_heads, total] (fp32), which packed_attention_backward takes.  Rows
-    outside every sequence are 0, or with `out` stay as they are there (lse
-    there: undefined)."""
+    [n_heads, total] (fp32), which packed_attention_backward takes, and with
+    return_residual what rounding took from a bf16 or fp16 output, in its type
+    (None in fp32), which makes the gradients of q and k there more exact.
+    Rows outside every sequence are 0, or with `out` stay as they are there
+    (lse and residual there: undefined)."""
     dt, q, k, v, cu = _packed_checks(q, k, v, cu_seqlens)
     total, H, D = q.shape
     fresh = out is None
     out = _fresh_or(out, q.shape, q)
     lse = torch.empty((H, total), device=q.device, dtype=torch.float32) if return_lse else None
+    lo = torch.empty(q.shape, device=q.device, dtype=q.dtype) if return_residual and dt else None
     scale = _default_scale(D) if scale is None else float(scale)
     if total:
         _call("rac_packed_attention_dev", q, q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(),
-              lse.data_ptr() if lse is not None else None, cu.data_ptr(), cu.numel() - 1, total, H, k.size(1), D,
+              lo.data_ptr() if lo is not None else None, lse.data_ptr() if lse is not None else None, cu.data_ptr(), cu.numel() - 1, total, H, k.size(1), D,
               *_packed_tail(q, k, v), scale, int(fresh), dt)
-    return (out, lse) if return_lse else out
+    if not (return_lse or return_residual):
+        return out
+    return (out,) + ((lse,) if return_lse else ()) + ((lo,) if return_residual else ())
 
 
 def packed_attention_backward(grad_out: torch.Tensor, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
                               out: torch.Tensor, lse: torch.Tensor, cu_seqlens: torch.Tensor,
-                              scale: Optional[float] = None) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+                              scale: Optional[float] = None, residual: Optional[torch.Tensor] = None
+                              ) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
     """(dq, dk, dv) of packed_attention, contiguous and in q's dtype, from its
-    output and lse; 0 in rows outside every sequence.  The sums over the query
+    output, lse and (may be None) residual; 0 in rows outside every sequence.  The sums over the query
     heads of a group run in a fixed order: the same call, the same bits."""
     dt, q, k, v, cu = _packed_checks(q, k, v, cu_seqlens)
     total, H, D = q.shape
-    for t, n in ((grad_out, "grad_out"), (out, "out")):
+    for t, n in ((grad_out, "grad_out"), (out, "out"), (residual, "residual")):
+        if t is None and n == "residual":
+            continue
         _like(t, q, n)
         if t.shape != q.shape or t.dtype != q.dtype:
             raise RuntimeError(f"RAC: {n} must have q's shape and dtype")
@@ -1190,6 +1199,7 @@ def packed_attention_backward(grad_out: torch.Tensor, q: torch.Tensor, k: torch.
     if lse.dtype != torch.float32 or tuple(lse.shape) != (H, total) or not lse.is_contiguous():
         raise RuntimeError("RAC: lse must be the contiguous fp32 [n_heads, total] of packed_attention")
     grad_out, out = grad_out.contiguous(), out.contiguous()
+    lo = residual.contiguous() if residual is not None else None
     dq = torch.empty(q.shape, device=q.device, dtype=q.dtype)
     dk, dv = (torch.empty(k.shape, device=q.device, dtype=q.dtype) for _ in range(2))
     scale = _default_scale(D) if scale is None else float(scale)
@@ -1197,7 +1207,7 @@ def packed_attention_backward(grad_out: torch.Tensor, q: torch.Tensor, k: torch.
         n = _lib.load().rac_packed_attention_backward_workspace_bytes(cu.numel() - 1, total, H, k.size(1), D)
         ws = torch.empty(n // 4, device=q.device, dtype=torch.float32)
         _call("rac_packed_attention_backward_dev", q, q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(),
-              grad_out.data_ptr(), lse.data_ptr(), cu.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(),
+              lo.data_ptr() if lo is not None else None, grad_out.data_ptr(), lse.data_ptr(), cu.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(),
               ws.data_ptr(), cu.numel() - 1, total, H, k.size(1), D, *_packed_tail(q, k, v), scale, 1, dt)
     return dq, dk, dv
 

@@ -827,16 +827,16 @@ class RACPackedAttentionFunction(Function):
         _need_gpu(q, "q")
         if not any(ctx.needs_input_grad[:3]):
             return _rac.packed_attention(q, k, v, cu_seqlens, scale)
-        out, lse = _rac.packed_attention(q, k, v, cu_seqlens, scale, return_lse=True)
-        ctx.save_for_backward(q, k, v, out, lse, cu_seqlens)
+        out, lse, lo = _rac.packed_attention(q, k, v, cu_seqlens, scale, return_lse=True, return_residual=True)
+        ctx.save_for_backward(q, k, v, out, lse, lo, cu_seqlens)
         ctx.scale = scale
         return out
 
     @staticmethod
     @once_differentiable
     def backward(ctx, g):
-        q, k, v, out, lse, cu_seqlens = ctx.saved_tensors
-        return (*_rac.packed_attention_backward(g, q, k, v, out, lse, cu_seqlens, ctx.scale), None, None)
+        q, k, v, out, lse, lo, cu_seqlens = ctx.saved_tensors
+        return (*_rac.packed_attention_backward(g, q, k, v, out, lse, cu_seqlens, ctx.scale, lo), None, None)
 
 
 def rac_packed_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqlens: torch.Tensor,

@@ -41,8 +41,8 @@ def make(lens, H, G, d, dt, seed=0, extra=0, start=0):
 
 def run(q, k, v, g, cu, scale=None):
     from rac_amd import ext
-    out, lse = ext.packed_attention(q, k, v, cu, scale, return_lse=True)
-    dq, dk, dv = ext.packed_attention_backward(g, q, k, v, out, lse, cu, scale)
+    out, lse, lo = ext.packed_attention(q, k, v, cu, scale, return_lse=True, return_residual=True)
+    dq, dk, dv = ext.packed_attention_backward(g, q, k, v, out, lse, cu, scale, lo)
     return dict(out=out, lse=lse, dq=dq, dk=dk, dv=dv)
 
 
@@ -220,6 +220,32 @@ def test_rows_outside_the_sequences(dt):
     res = ext.packed_attention(q, k, v, cu, out=kept)
     assert res is kept and bool((kept[:start] == 7).all()) and bool((kept[start + 93:] == 7).all())
     assert torch.equal(kept[start:start + 93], got["out"][start:start + 93])
+
+
+@pytest.mark.parametrize("dt", [BF16, F16])
+@pytest.mark.parametrize("d", [64, 33])
+def test_the_residual_of_a_rounded_output(dt, d):
+    """out + residual is the output to the sums' own error: its bound without
+    the output's rounding, half a step of what rounding can take away besides.
+    The gradients hold their bounds without it, and with it a bound whose D has
+    only the residual's error."""
+    from rac_amd import ext
+    lens = [90, 41]
+    q, k, v, g = make(lens, 4, 2, d, dt)
+    cu = cu_of(lens)
+    out, lse, lo = ext.packed_attention(q, k, v, cu, return_lse=True, return_residual=True)
+    want, tol = ref.packed_reference(q, k, v, lens, 1 / math.sqrt(d), g)
+    u = ref.half_step(dt)
+    fine = tol["out"] - u * want["out"].abs() + u * u * want["out"].abs() + 2.0 ** -25
+    ref.check(out.double() + lo.double(), want["out"], fine, "out + residual")
+    assert bool((lo.double().abs().cpu() <= u * 1.01 * out.double().abs().cpu() + 2.0 ** -25).all())
+    without = dict(zip(("dq", "dk", "dv"), ext.packed_attention_backward(g, q, k, v, out, lse, cu)))
+    compare(without, want, tol, names=("dq", "dk", "dv"))
+    wide = torch.full((131, 4, d + 1), float("nan"), device=DEV, dtype=dt)[..., 1:]
+    wide.copy_(lo)
+    both = [ext.packed_attention_backward(g, q, k, v, out, lse, cu, residual=x) for x in (lo, wide)]
+    assert all(torch.equal(a, b) for a, b in zip(*both))
+    assert ext.packed_attention(q.float(), k.float(), v.float(), cu, return_residual=True)[1] is None
 
 
 def test_no_sequences_and_no_rows():
