@@ -237,16 +237,22 @@ __device__ __forceinline__ bool not_finite(const f32x16 (&acc)[N]) {
     return t != 0.0f;                   // NaN
 }
 
+// The wave's columns (bit r: column r) of which a lane says so.
+__device__ __forceinline__ uint32_t columns_of(bool lane_says) {
+    const uint64_t b = __ballot(lane_says);
+    return (uint32_t)b | (uint32_t)(b >> 32);
+}
+
 // dot product of two rows of d values, and its partner's values times f added
 // to lane e's columns e, e + 64, ...: the parts of a row done again on the VALU
 template <typename T>
-__device__ float row_dot(const T* x, const T* y, int d) {
+__device__ __forceinline__ float row_dot(const T* x, const T* y, int d) {
     float s = 0.0f;
     for (int c = 0; c < d; c++) s = __builtin_fmaf(Mma<T>::to_f32(x[c]), Mma<T>::to_f32(y[c]), s);
     return s;
 }
 template <typename T, int DP>
-__device__ void row_axpy(float (&acc)[(DP + 63) / 64], float f, const T* y, int d) {
+__device__ __forceinline__ void row_axpy(float (&acc)[(DP + 63) / 64], float f, const T* y, int d) {
 #pragma unroll
     for (int n = 0; n < (DP + 63) / 64; n++) {
         const int c = (threadIdx.x & 63) + 64 * n;
@@ -257,7 +263,7 @@ __device__ void row_axpy(float (&acc)[(DP + 63) / 64], float f, const T* y, int 
 // one to a lane, then their rows one by one; nothing of a j outside is read
 // (with SKIP, nor of a j whose weight is below 0)
 template <typename T, int DP, bool SKIP = false, typename O, typename W, typename R>
-__device__ void attn_again(O* out, float f, int d, int j0, int j1, W w, R rows, O* lo = nullptr) {
+__device__ __forceinline__ void attn_again(O* out, float f, int d, int j0, int j1, W w, R rows, O* lo = nullptr) {
     float acc[(DP + 63) / 64] = {};
     for (int j = j0; j < j1; j += 64) {
         const int mine = j + (threadIdx.x & 63);

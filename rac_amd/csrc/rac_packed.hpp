@@ -24,7 +24,8 @@
 // infinities among them: masked scores are replaced before the exponential;
 // where a tile's product would still multiply such a value by a probability of
 // 0, the row's accumulators show it (they are not finite), and its wave does
-// that row again over the keys it sees and no others (attn_again).
+// that row again over the keys it sees and no others (attn_again).  A row whose
+// own weights are NaN is NaN throughout and stays so.
 #pragma once
 #include <hip/hip_runtime.h>
 #include "rac_internal.hpp"

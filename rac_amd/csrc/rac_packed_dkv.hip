@@ -164,15 +164,14 @@ __global__ __launch_bounds__(kPkThreads, DP * sizeof(T) <= 128 ? 2 : 1) void pac
     bool bad = false;
     if constexpr (WK) bad |= not_finite(ak);
     if constexpr (WV) bad |= not_finite(av);
-    uint64_t again = __ballot(bad && there);
-    again = (again | again >> 32) & 0xffffffffull;
+    uint32_t again = columns_of(bad && there);
     if (there && !(again >> (lane & 31) & 1)) {
         const long at = (row * oheads + h) * a.d;
         if constexpr (WK) attn_store<O, ND>(dk + at, ak, a.scale, a.d, half, BY_HEAD ? a.d % 4 == 0 : a.vec_out);
         if constexpr (WV) attn_store<O, ND>(dv + at, av, 1.0f, a.d, half, BY_HEAD ? a.d % 4 == 0 : a.vec_out);
     }
     for (; again; again &= again - 1) {
-        const int kr = kw + __ffsll((unsigned long long)again) - 1, from = kr, n = seg.len - from;
+        const int kr = kw + __ffs((int)again) - 1, from = kr, n = seg.len - from;
         const long at = ((long)(seg.start + kr) * oheads + h) * a.d;
         const T* kk = (const T*)a.k + (long)(seg.start + kr) * a.sk_t + (long)g * a.sk_h;
         const T* vv = (const T*)a.v + (long)(seg.start + kr) * a.sv_t + (long)g * a.sv_h;
@@ -181,10 +180,16 @@ __global__ __launch_bounds__(kPkThreads, DP * sizeof(T) <= 128 ? 2 : 1) void pac
         auto grow = [&](int i) { return G + ((long)(from + i % n) * a.heads + i / n) * a.d; };
         auto stats_of = [&](int i) { return a.stats + 2 * ((long)(h0 + i / n) * a.total + seg.start + from + i % n); };
         auto prob = [&](int i) { return exp2_hw(__builtin_fmaf(row_dot(qrow(i), kk, a.d), c, -*stats_of(i))); };
-        if constexpr (WV) attn_again<T, DP>(dv + at, 1.0f, a.d, 0, n * rep, prob, grow);
-        if constexpr (WK)
-            attn_again<T, DP>(dk + at, a.scale, a.d, 0, n * rep,
-                                [&](int i) { return prob(i) * (row_dot(grow(i), vv, a.d) - stats_of(i)[1]); }, qrow);
+        auto score = [&](int i) { return prob(i) * (row_dot(grow(i), vv, a.d) - stats_of(i)[1]); };
+        // a NaN weight of the key's own query: no head to sum over
+        if constexpr (WV) {
+            const float w = prob(0);
+            attn_again<T, DP>(dv + at, w == w ? 1.0f : w, a.d, 0, w == w ? n * rep : 0, prob, grow);
+        }
+        if constexpr (WK) {
+            const float w = score(0);
+            attn_again<T, DP>(dk + at, w == w ? a.scale : w, a.d, 0, w == w ? n * rep : 0, score, qrow);
+        }
     }
 }
 

@@ -127,13 +127,11 @@ __global__ __launch_bounds__(kPkThreads, DP * sizeof(T) <= 256 ? 2 : 1) void pac
         join_groups<KG, WR, ND>(acc, 1.0f, ka, wr, kg, lane);
         if (kg) return;
     }
-    const bool bad = not_finite(acc) && there;
-    uint64_t again = __ballot(bad);
-    again = (again | again >> 32) & 0xffffffffull;
+    uint32_t again = columns_of(not_finite(acc) && there && lse == lse && dl == dl);
     if (there && !(again >> (lane & 31) & 1))
         attn_store<T, ND>(dq + (row * a.heads + h) * a.d, acc, a.scale, a.d, half, a.vec_out);
     for (; again; again &= again - 1) {
-        const int r = __ffsll((unsigned long long)again) - 1;
+        const int r = __ffs((int)again) - 1;
         const long t = qw + r, at = ((seg.start + t) * a.heads + h) * a.d;
         const float lr = __shfl(lse, r), dr = __shfl(dl, r);
         const T* q = (const T*)a.q + (seg.start + t) * a.sq_t + (long)h * a.sq_h;

@@ -140,9 +140,7 @@ __global__ __launch_bounds__(kPkThreads, DP * sizeof(T) <= 256 ? 2 : 1) void pac
         if (kg) return;
     }
     const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-    const bool bad = not_finite(o) && qrow < seg.len;
-    uint64_t again = __ballot(bad);
-    again = (again | again >> 32) & 0xffffffffull;
+    uint32_t again = columns_of(not_finite(o) && qrow < seg.len && l == l);
     if (qrow < seg.len) {
         const long row = seg.start + qrow;
         const long at = (row * a.heads + h) * a.d;
@@ -153,7 +151,7 @@ __global__ __launch_bounds__(kPkThreads, DP * sizeof(T) <= 256 ? 2 : 1) void pac
         if (a.lse && half == 0) a.lse[(long)h * a.total + row] = (m + __builtin_amdgcn_logf(l)) * kLn2;
     }
     for (; again; again &= again - 1) {
-        const int r = __ffsll((unsigned long long)again) - 1, t = qw + r;
+        const int r = __ffs((int)again) - 1, t = qw + r;
         const float mr = __shfl(m, r), ir = __shfl(inv, r);
         const T* q = (const T*)a.q + (long)(seg.start + t) * a.sq_t + (long)h * a.sq_h;
         const long at = ((long)(seg.start + t) * a.heads + h) * a.d;

@@ -229,9 +229,9 @@ __global__ __launch_bounds__(kTreeThreads, DP * sizeof(T) <= 256 ? 2 : 1) void t
         m = mt;
         if (kg) return;
     }
-    // rows that met a value that is not finite: again, over what they see
-    uint64_t again = __ballot(not_finite(o) && there);
-    again = (again | again >> 32) & 0xffffffffull;
+    // rows that met a value that is not finite in a split with drafts, which may
+    // be one they do not see: again, over what they do
+    uint32_t again = j1 * TILE > len ? columns_of(not_finite(o) && there && l == l) : 0;
     const bool store = there && !(again >> (lane & 31) & 1);
     const float inv = l == 0.0f ? 0.0f : 1.0f / l;
     const bool whole = per >= tiles;                      // no other split has keys
@@ -248,7 +248,7 @@ __global__ __launch_bounds__(kTreeThreads, DP * sizeof(T) <= 256 ? 2 : 1) void t
         if (store) attn_store<float, ND>(po + (long)r * a.d, o, 1.0f, a.d, half, a.d % 4 == 0);
     }
     for (; again; again &= again - 1) {
-        const int rl = __ffsll((unsigned long long)again) - 1, rr = rw + rl;
+        const int rl = __ffs((int)again) - 1, rr = rw + rl;
         const int t = rr / rep, hh = g * rep + rr % rep;
         const float mr = __shfl(m, rl), ir = __shfl(inv, rl);
         const T* q = (const T*)a.q + (long)b * a.sq_b + (long)t * a.sq_t + (long)hh * a.sq_h;

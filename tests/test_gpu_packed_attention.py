@@ -161,6 +161,33 @@ def test_values_a_row_does_not_see(dt, bad, which):
 
 
 @pytest.mark.parametrize("dt", [F32, BF16])
+@pytest.mark.parametrize("heads", [2, 64])
+def test_seen_and_unseen_values_that_are_not_finite(dt, heads):
+    """An early token's NaN reaches the rows behind it in its own column only,
+    whatever a later token, in the tiles on those rows' diagonals, holds (two
+    head counts: one and four row sets to a workgroup in the longer sequence)."""
+    lens, d = [700], 64
+    q, k, v, g = make(lens, heads, 1, d, dt)
+    v[10, 0, 7] = float("nan")
+    v[650, 0, 3] = float("inf")
+    k[651, 0, 5] = float("nan")
+    out = run(q, k, v, g, cu_of(lens))["out"]
+    clean = make(lens, heads, 1, d, dt)
+    want, tol = ref.packed_reference(clean[0][:, :2], clean[1], clean[2], lens, 1 / math.sqrt(d))
+    rest = [c for c in range(d) if c != 7]
+    assert bool(out[10:, :, 7].isnan().all()) and not bool(out[:650, :, rest].isnan().any())
+    ref.check(out[:650, :2][..., rest], want["out"][:650][..., rest], tol["out"][:650][..., rest], "out")
+    g[655, :, 9] = float("nan")                      # and a late row's gradient the keys before it only
+    got = run(*clean[:3], g, cu_of(lens))
+    want, tol = ref.packed_reference(clean[0][:, :2], clean[1], clean[2], lens, 1 / math.sqrt(d), clean[3][:, :2])
+    assert bool(got["dv"][:656, :, 9].isnan().all()) and not bool(got["dv"][656:].isnan().any())
+    assert not bool(got["dv"][:, :, :9].isnan().any())
+    if heads == 2:
+        for n in ("dk", "dv"):
+            ref.check(got[n][656:], want[n][656:], tol[n][656:], n)
+
+
+@pytest.mark.parametrize("dt", [F32, BF16])
 def test_nan_reaches_what_it_should(dt):
     lens, d, at = [150], 64, 100
     q, k, v, g = make(lens, 2, 1, d, dt)
@@ -170,6 +197,17 @@ def test_nan_reaches_what_it_should(dt):
     assert not bool(got["out"][at:, :, :7].isnan().any())
     v[at, 0, 7] = float("inf")
     assert bool((run(q, k, v, g, cu_of(lens))["out"][at:, :, 7] == float("inf")).all())
+
+
+@pytest.mark.parametrize("dt", [F32, BF16])
+def test_nothing_but_nan(dt):
+    lens = [300, 40]
+    q, k, v, g = make(lens, 4, 2, 64, dt)
+    for t in (q, k, v, g):
+        t[:300] = float("nan")
+    got = run(q, k, v, g, cu_of(lens))
+    for n in ("out", "dq", "dk", "dv"):
+        assert bool(got[n][:300].isnan().all()) and not bool(got[n][300:].isnan().any()), n
 
 
 def test_scores_of_minus_infinity():
