@@ -16,6 +16,7 @@
  * Strides count elements; d_head values of a head are contiguous.  Rows that
  * start on 16-byte boundaries and whose d_head is a multiple of 16 bytes are
  * read 16 bytes at a time, others value by value, with the same results.
+ * Outputs and workspaces overlap no input.
  */
 #ifndef RAC_LLM_H
 #define RAC_LLM_H
@@ -42,7 +43,7 @@ extern "C" {
  * Rows of out outside every sequence become 0 with zero_rest and stay as they
  * are without; their lse stays as it is.  A row whose scores are all -inf gives
  * 0; values at positions a row does not see never reach it, NaN included.
- * scale > 0; total <= 2^30. */
+ * scale > 0; total <= 2^30 and (total / 32 + n_seqs + 2) * n_heads < 2^24. */
 int rac_packed_attention_dev(const void *q, const void *k, const void *v, void *out, void *out_lo, float *lse,
                              const int *cu_seqlens, int n_seqs, int total, int n_heads, int n_kv_heads, int d_head,
                              long q_stride, long q_head_stride, long k_stride, long k_head_stride, long v_stride,
@@ -75,7 +76,8 @@ int rac_packed_attention_backward_dev(const void *q, const void *k, const void *
  * kernels run, so a recorded graph replays with new ones.  A sequence whose
  * lengths[b] is not in [0, t_cap - tokens] gives NaN and reads no cache.
  * parents_stride 0: one tree for all.  1 <= tokens <= 256; batch * n_kv_heads
- * <= 65535.  workspace: rac_tree_attention_workspace_bytes bytes (null when
+ * <= 65535, and times the 32-row blocks of a key head's queries below 2^24 -
+ * 4096.  workspace: rac_tree_attention_workspace_bytes bytes (null when
  * that is 0), the call's own while it runs. */
 long rac_tree_attention_workspace_bytes(int batch, int tokens, int n_heads, int n_kv_heads, int d_head, long t_cap,
                                         int dtype);
@@ -92,7 +94,7 @@ int rac_tree_attention_dev(const void *q, const void *k_cache, const void *v_cac
  * log probabilities [rows, top].  tokens (64-bit): a negative one stands for
  * none (logprob 0), one >= vocab gives NaN.  A row of nothing but -inf has log
  * probabilities -inf and entropy 0; NaN or +inf in a row makes its results NaN.
- * vocab < 2^31; top <= min(64, vocab).  workspace:
+ * rows < 2^24, vocab < 2^31 - 64; top <= min(64, vocab).  workspace:
  * rac_token_logprobs_workspace_bytes bytes (null when that is 0). */
 long rac_token_logprobs_workspace_bytes(long rows, long vocab, int top, int dtype);
 int rac_token_logprobs_dev(const void *logits, long row_stride, const long *tokens, float *logprob, float *entropy,

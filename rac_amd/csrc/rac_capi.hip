@@ -470,6 +470,9 @@ RAC_EXPORT int rac_softmax_dev(const float* x, float* y, long rows, long n, int 
 
 // ── packed prompts, drafted tokens, given tokens (rac_llm.h) ────────────
 
+// workgroups of 256 threads that a launch takes: it counts threads in 32 bits
+constexpr long kLlmMaxGroups = (1L << 24) - 1;
+
 static bool rows_aligned(const void* p, int es, int d, long s0, long s1, long s2 = 0) {
     const long v = 16 / es;
     return (uintptr_t)p % 16 == 0 && d % v == 0 && s0 % v == 0 && s1 % v == 0 && s2 % v == 0;
@@ -491,7 +494,7 @@ static int packed_args(const char* who, PackedArgs* a, int dtype) {
     if (rc) return rc;
     if (a->n_seqs < 0 || a->total < 0 || a->total > (1 << 30))
         return fail(RAC_ERR_INVALID_DIM, "%s: n_seqs and total must not be negative, total at most 2^30", who);
-    if (((long)a->total / 32 + a->n_seqs + 2) * a->heads > 2147483647L)
+    if (((long)a->total / 32 + a->n_seqs + 2) * a->heads > kLlmMaxGroups)
         return fail(RAC_ERR_INVALID_DIM, "%s: too many sequences and heads", who);
     if (a->sq_t < 0 || a->sq_h < 0 || a->sk_t < 0 || a->sk_h < 0 || a->sv_t < 0 || a->sv_h < 0)
         return fail(RAC_ERR_INVALID_DIM, "%s: strides must not be negative", who);
@@ -572,8 +575,8 @@ static int tree_args(const char* who, const TreeArgs& a, int dtype) {
         return fail(RAC_ERR_INVALID_DIM, "%s: tokens must be in [1, %d]", who, kTreeMaxTokens);
     if (a.cap < a.tokens || a.cap > 2147483647L - 65536)
         return fail(RAC_ERR_INVALID_DIM, "%s: t_cap must hold the tokens and stay below 2^31 - 65536", who);
-    // at most 64 splits of the keys
-    if (64L * (a.batch * (long)a.kv_heads + 8) * ((long)a.heads / a.kv_heads * a.tokens / 32 + 1) > 2147483647L)
+    // splits add at most two workgroups for every CU to one for each block of rows
+    if (((long)a.batch * a.kv_heads + 8) * ((long)a.heads / a.kv_heads * a.tokens / 32 + 1) > kLlmMaxGroups - 4096)
         return fail(RAC_ERR_INVALID_DIM, "%s: too many query rows", who);
     return RAC_OK;
 }
@@ -622,7 +625,7 @@ RAC_EXPORT int rac_tree_attention_dev(const void* q, const void* k_cache, const 
 }
 
 static int check_logits(const char* who, long rows, long vocab, long row_stride, int dtype) {
-    if (rows < 0 || rows > 2147483647L) return fail(RAC_ERR_INVALID_DIM, "%s: rows must be in [0, 2^31 - 1]", who);
+    if (rows < 0 || rows > kLlmMaxGroups) return fail(RAC_ERR_INVALID_DIM, "%s: rows must be in [0, 2^24 - 1]", who);
     if (vocab < 1 || vocab > 2147483647L - 64) return fail(RAC_ERR_INVALID_DIM, "%s: vocab must be in [1, 2^31 - 65]", who);
     if (row_stride < vocab && rows > 1)
         return fail(RAC_ERR_INVALID_DIM, "%s: row_stride must be at least vocab", who);

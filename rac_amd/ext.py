@@ -1108,6 +1108,19 @@ def _fresh_or(out: Optional[torch.Tensor], shape, ref: torch.Tensor) -> torch.Te
     return out
 
 
+def _apart(out: Optional[torch.Tensor], *ins: torch.Tensor) -> None:
+    """Refuses a given out that shares memory with an input."""
+    if out is None or not out.numel():
+        return
+    lo = out.data_ptr()
+    hi = lo + out.numel() * out.element_size()
+    for t in ins:
+        first = t.data_ptr()
+        last = first + sum((n - 1) * s for n, s in zip(t.shape, t.stride())) * t.element_size()
+        if t.numel() and lo <= last + t.element_size() - 1 and first < hi:
+            raise RuntimeError("RAC: out must not share memory with an input")
+
+
 def _call(name: str, ref: torch.Tensor, *args) -> None:
     """The entry point on ref's device and torch's current stream there."""
     index = ref.device.index
@@ -1162,11 +1175,13 @@ def packed_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqle
     [n_heads, total] (fp32), which packed_attention_backward takes, and with
     return_residual what rounding took from a bf16 or fp16 output, in its type
     (None in fp32), which makes the gradients of q and k there more exact.
-    Rows outside every sequence are 0, or with `out` stay as they are there
-    (lse and residual there: undefined)."""
+    Rows outside every sequence are 0, or with `out` (which shares no memory
+    with an input) stay as they are there (lse and residual there:
+    undefined)."""
     dt, q, k, v, cu = _packed_checks(q, k, v, cu_seqlens)
     total, H, D = q.shape
     fresh = out is None
+    _apart(out, q, k, v, cu)
     out = _fresh_or(out, q.shape, q)
     lse = torch.empty((H, total), device=q.device, dtype=torch.float32) if return_lse else None
     lo = torch.empty(q.shape, device=q.device, dtype=q.dtype) if return_residual and dt else None
@@ -1224,7 +1239,8 @@ def tree_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor
     itself.  parents [T] is one tree for all.  lengths and parents (int32) are
     read on the device when the kernels run: a recorded graph replays with new
     ones.  Without the batch dim (q [T, n_heads, d_head], caches [n_kv_heads,
-    t_cap, d_head], one length): one sequence.  T <= 256.  Returns q's shape;
+    t_cap, d_head], one length): one sequence.  T <= 256.  A given out shares
+    no memory with an input.  Returns q's shape;
     NaN for a sequence whose length does not leave T positions."""
     single = isinstance(q, torch.Tensor) and q.dim() == 3
     dt = _llm_dtype(q, "q")
@@ -1253,6 +1269,7 @@ def tree_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor
     if tuple(parents.shape) not in ((T,), (B, T)):
         raise RuntimeError("RAC: parents must be [T] or [batch, T]")
     q, k, v = _unit_last(q), _unit_last(k_cache), _unit_last(v_cache)
+    _apart(out, q, k, v, lengths, parents)
     res = _fresh_or(out, (T, H, D) if single else (B, T, H, D), q)
     scale = _default_scale(D) if scale is None else float(scale)
     if B:

@@ -70,6 +70,13 @@ def test_packed_arguments(lib, bad):
     assert packed(lib, **bad) == -2 and backward(lib, **bad) == -2
 
 
+def test_more_workgroups_than_a_launch_counts(lib):
+    assert packed(lib, total=2 ** 28, H=4, G=2) == -2 and packed(lib, n=2 ** 24, H=2, G=1) == -2
+    assert backward(lib, total=2 ** 28, H=4, G=2) == -2
+    assert tree(lib, B=65535, G=1, H=128, T=256) == -2       # 65535 x 1024 blocks of 32 rows
+    assert logp(lib, rows=2 ** 24) == -2 and logp_backward(lib, rows=2 ** 24) == -2
+
+
 def test_null_buffers(lib):
     for n in ("q", "k", "v", "out", "cu"):
         assert packed(lib, **{n: None}) == -1
@@ -187,3 +194,29 @@ def test_python_refuses_shapes_and_types():
         with pytest.raises(RuntimeError):
             ext.token_logprobs_backward(x, tok, *args)
     assert bool((ext.token_logprobs_backward(x, tok, lse, ent, None, None) == 0).all())
+
+
+@pytest.mark.gpu
+def test_an_output_within_an_input():
+    from rac_amd import ext
+    if not torch.cuda.is_available():
+        pytest.skip("no ROCm device")
+    D = "cuda"
+    flat = torch.randn(5, 12, 64, device=D)
+    q, k, v = flat[:, :4], flat[:, 4:8], flat[:, 8:]
+    cu = torch.tensor([0, 5], dtype=torch.int32, device=D)
+    plain = ext.packed_attention(q, k, v, cu)
+    for t in (q.contiguous(), v.contiguous()):
+        with pytest.raises(RuntimeError, match="share"):
+            ext.packed_attention(t, k, t, cu, out=t)
+    with pytest.raises(RuntimeError, match="share"):
+        ext.packed_attention(q, k, v, cu, out=flat.view(-1)[-5 * 256:].view(5, 4, 64))
+    both = torch.empty(2 * 5 * 256, device=D)                 # neighbours in one buffer are no overlap
+    own = both[:1280].view(5, 4, 64).copy_(q)
+    out = ext.packed_attention(own, k, v, cu, out=both[1280:].view(5, 4, 64))
+    assert torch.equal(out, plain)
+    t, c = torch.randn(1, 3, 4, 64, device=D), torch.randn(1, 4, 9, 64, device=D)
+    par = torch.tensor([-1, 0, 1], dtype=torch.int32, device=D)
+    for o in (t, c.view(-1)[:768].view(1, 3, 4, 64)):
+        with pytest.raises(RuntimeError, match="share"):
+            ext.tree_attention(t, c, c, cu[1:], par, out=o)
