@@ -185,7 +185,10 @@ __device__ __forceinline__ void lp_finish(const LogprobArgs& a, long row, const 
 // floats of a split's part: three statistics, a gap, `top` entries
 __host__ __device__ constexpr int lp_width(int top) { return 4 + 2 * top; }
 
-// One workgroup per row and split: columns [c0, c1) of the row.
+// One workgroup per row and split: vectors [v0, v1) of the row.  Bound by reading
+// the logits: 2048 bf16 rows of 128000 with 5 alternatives 121 us (4.3 TB/s;
+// without 109, 4.8), 1001 fp32 rows of 50001 36 us in two launches.  One batch of
+// loads is under way while the one before is summed (130 us in graph replay, loaded where used 153).
 template <typename T, bool TOP>
 __global__ __launch_bounds__(kLpThreads) void logprob_kernel(const LogprobArgs a) {
     constexpr int VEC = Mma<T>::VEC, U = 4;                // U vectors of a thread in flight
@@ -379,7 +382,10 @@ __global__ __launch_bounds__(kLpThreads) void logprob_join_kernel(const LogprobA
     lp_finish<T>(a, row, r, best);
 }
 
-// dx of a piece of a row: VEC values a thread and step.
+// dx of a piece of a row: VEC values a thread and step, four steps.  Reads the
+// logits and writes as much: 1001 fp32 rows of 50001 84 us, 4096 bf16 rows of
+// 32000 110 (4.7 TB/s both, a large copy's rate).  One step to a thread 85 and
+// 113, sixteen 87 and 109, and 64 bf16 rows of 32000 4.1 and 10.2 against 4.9.
 template <typename T>
 __global__ __launch_bounds__(kLpThreads) void logprob_backward_kernel(const void* __restrict__ xv, long stride,
                                                                      const long* __restrict__ tok,
@@ -430,10 +436,14 @@ __global__ __launch_bounds__(kLpThreads) void logprob_backward_kernel(const void
     }
 }
 
-// Workgroups of few rows: about four to a CU, each of at least 2048 values.
+// Workgroups of few rows: about two to a CU, each of at least 4096 values.  us
+// without alternatives, with 20 in the first two (MI355X), in two to a CU, four
+// and one: 16 bf16 rows of 128000 21.4, 25, 18.9; 4 fp32 rows of 32000 14.5 in
+// each; 64 fp32 rows of 128000 10.9, 11.2, 12.5; 1001 fp32 rows of 50001 36, 38,
+// 36.  In pieces of 2048 at least the 4 rows take 15.7, in 8192 18.2.
 static int logprob_splits(long rows, long vocab) {
-    long s = (4 * device_cus() + rows - 1) / rows;
-    const long most = (vocab + 2047) / 2048;
+    long s = (2 * device_cus() + rows - 1) / rows;
+    const long most = (vocab + 4095) / 4096;
     if (s > most) s = most;
     return s < 1 ? 1 : (int)s;
 }

@@ -4,6 +4,12 @@
 
 namespace rac {
 
+// p and ds of 32 keys as columns, then dv += p do and dk += ds q: four products
+// of a tile of q and do, each read both ways, over the group's query heads.  Both
+// sums' accumulators and the keys' fragments leave a SIMD one wave in rows of 256
+// bytes, whose matrix instructions wait for its own LDS reads (busy 0.28): six
+// bf16 documents of 8192 rows (32/8 heads of 128) 568 - 627 us, fp32 rows of
+// 777, 1, 1250 and 63 (12/4 heads of 80, by query head) 141 and the join 7.
 // WHICH: 1 dv, 2 dk, 3 both (d past 128 in fp32 has no registers for both)
 // BY_HEAD: a workgroup sums one query head's part, in fp32, for the join below
 template <typename T, int DP, int WR, int WHICH, bool BY_HEAD>

@@ -3,6 +3,11 @@
 
 namespace rac {
 
+// Bound by matrix instructions and, in 16 bits, the exponentials beside them,
+// which one wave's products and another's softmax overlap: two workgroups to a
+// CU.  One bf16 prompt of 8192 (32/8 heads of 128) 521 - 558 us, 1.0 PFLOP/s of
+// the triangle, matrix cores busy 0.57 of the time and the VALU 0.51; six fp32
+// prompts of 4096 rows in all (32/4 heads of 64) 225 us, matrix cores 0.77.
 template <typename T, int DP, int WR>
 __global__ __launch_bounds__(kPkThreads, DP * sizeof(T) <= 256 ? 2 : 1) void packed_fwd_kernel(const PackedArgs a) {
     using M = Mma<T>;
