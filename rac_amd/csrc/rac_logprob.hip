@@ -187,8 +187,9 @@ __host__ __device__ constexpr int lp_width(int top) { return 4 + 2 * top; }
 
 // One workgroup per row and split: vectors [v0, v1) of the row.  Bound by reading
 // the logits: 2048 bf16 rows of 128000 with 5 alternatives 121 us (4.3 TB/s;
-// without 109, 4.8), 1001 fp32 rows of 50001 36 us in two launches.  One batch of
-// loads is under way while the one before is summed (130 us in graph replay, loaded where used 153).
+// without 109, 4.8), 1001 fp32 rows of 50001 36 us (5.5 TB/s, part
+// of it from cache).  One batch of loads is under way while the one before is
+// summed (130 us in graph replay; loaded where used 153).
 template <typename T, bool TOP>
 __global__ __launch_bounds__(kLpThreads) void logprob_kernel(const LogprobArgs a) {
     constexpr int VEC = Mma<T>::VEC, U = 4;                // U vectors of a thread in flight
