@@ -25,7 +25,7 @@
 // each by half a step of its own value and independently of the others, because
 // the matrix cores take 16-bit operands at seven times the fp32 rate: relative
 // to their size, bf16 outputs are off by 0.0021 and dq by 0.0027 in all, of which
-// the rounding of the results themselves is 0.0017. 
+// the rounding of the results themselves is 0.0017.
 //
 // Values in places the mask takes away do not reach a result, NaN and
 // infinities among them: masked scores are replaced before the exponential;
